@@ -252,6 +252,115 @@ int em_attention(const em_attention_shape* s, size_t rows, const int* pos_dev, c
                  const float* key_cache, const float* value_cache, float* out, float* scratch,
                  int kernel, void* stream);
 
+/* ---- A paged KV cache of many sequences ----------------------------------
+ * Keys and values of many sequences in pages of page_size positions. A batch
+ * of rows (tokens) is described by device arrays, so a captured graph serves
+ * every step: sequence s owns rows [row_start[s], row_start[s + 1]), of which
+ * row r is at position lengths[s] - (row_start[s + 1] - r), lengths[s] counting
+ * the batch's own rows. Position t of the sequence is slot t % page_size of
+ * page page_table[s * table_stride + t / page_size]. row_start must not fall;
+ * a sequence may have no rows. Rows outside [row_start[0], row_start[n_seqs])
+ * (a padded batch) are nobody's: no operator writes anything for them.
+ * Positions that do not exist (negative ones, those past max_pages *
+ * page_size) and pages outside [0, n_pages) hold nothing: nothing is stored
+ * there and attention does not see them. No counterpart in the reference,
+ * which has one sequence and one contiguous cache. */
+
+/* How the caches hold a value. 16-bit values are rounded to nearest even on
+ * the way in (fp16 past 65504 becomes an infinity); products and sums are fp32. */
+#define EM_CACHE_F32 0
+#define EM_CACHE_F16 1
+#define EM_CACHE_BF16 2
+
+/* Element (page, slot, kv head, d) of either cache is at page * page_stride +
+ * slot * slot_stride + kv head * head_stride + d. */
+typedef struct {
+    int n_heads, n_kv_heads, head_size; /* head_size a multiple of 8, at most 256 */
+    int page_size;                      /* positions a page, any number from 1 */
+    int n_pages;                        /* pages of each cache */
+    int max_pages;                      /* pages of a sequence: columns of the page table */
+    int type;                           /* EM_CACHE_* */
+    size_t page_stride, slot_stride, head_stride; /* elements, multiples of 8 */
+} em_paged_shape;
+
+typedef struct {
+    int n_seqs;
+    const int* row_start;  /* n_seqs + 1 */
+    const int* lengths;    /* n_seqs */
+    const int* page_table; /* n_seqs rows of max_pages */
+    size_t table_stride;   /* ints between its rows, at least max_pages */
+} em_paged_batch;
+
+/* EM_OK if the operators below can run shape s, else EM_EINVAL with the reason. */
+int em_paged_check(const em_paged_shape* s);
+
+/* Stores the keys and values of `rows` rows at their positions, the first
+ * `rotary` dims of each key and query head (a multiple of 8, 0 for none)
+ * rotated by them on the way: pair i by the angle position * freq[i] (rotary /
+ * 2 floats, device memory; the angle formed in 64 bits, its cosine and sine
+ * rounded to fp32 once), pair i being dims (2i, 2i + 1), the model's, or with
+ * halves != 0 dims (i, i + rotary / 2). Row r's queries (n_heads heads) are at
+ * q + r * q_stride, its keys and values (n_kv_heads) at k and v likewise, all
+ * fp32, e.g. columns of one qkv product; the rotated queries go to q_out +
+ * r * q_out_stride, which may be q itself. q NULL: keys and values alone.
+ * A row at a position that does not exist is left alone; one whose page holds
+ * nothing has its queries rotated. Two rows at one slot leave either's values.
+ * Pointers 16-byte aligned, row strides multiples of 4. */
+int em_paged_append(const em_paged_shape* s, const em_paged_batch* b, size_t rows, const float* q,
+                    size_t q_stride, const float* k, size_t k_stride, const float* v,
+                    size_t v_stride, const float* freq, int rotary, int halves, float* q_out,
+                    size_t q_out_stride, void* key_cache, void* value_cache, void* stream);
+
+/* Floats of scratch em_paged_attention needs for a batch of n_seqs sequences
+ * and `rows` rows in all (0 for a shape it cannot run). */
+size_t em_paged_attention_scratch_floats(const em_paged_shape* s, size_t n_seqs, size_t rows);
+
+/* Causal attention of each row over its sequence's cached positions, its own
+ * among them (append first): row r at position p and query head h see
+ * positions t <= p, with window > 0 those past p - window alone, of kv head
+ * h / (n_heads / n_kv_heads): out = sum_t softmax_t(scale * q . k_t) v_t. scale
+ * 0 is 1 / sqrt(head_size). Positions a row does not see never reach its
+ * output, whatever their slots hold. A row that sees nothing gets zeros.
+ * Scratch is the caller's, used by this call alone until it has run; it needs
+ * no zero fill. Results are bit-identical across calls of one shape, batch
+ * and row count. Pointers 16-byte aligned, row strides multiples of 4. */
+int em_paged_attention(const em_paged_shape* s, const em_paged_batch* b, size_t rows,
+                       const float* q, size_t q_stride, const void* key_cache,
+                       const void* value_cache, float* out, size_t out_stride, float scale,
+                       int window, float* scratch, void* stream);
+
+/* ---- Sampling --------------------------------------------------------------
+ * Settings of each row, device arrays of `rows`; a NULL array is that filter
+ * off (temperature NULL: 1). */
+typedef struct {
+    const float* temperature; /* <= 0 or NaN: the row's largest logit, whatever u is */
+    const int* top_k;         /* <= 0: off */
+    const float* top_p;       /* >= 1 or NaN: off; <= 0: the first alone */
+    const float* min_p;       /* <= 0 or NaN: off; > 1 counts as 1 */
+} em_sampling;
+
+/* Bytes of scratch em_sample needs (0 for a size it cannot run). */
+size_t em_sample_scratch_bytes(size_t rows, size_t vocab);
+
+/* The next token of each row of logits from the number u[r] in [0, 1):
+ *   weights     w_i = exp((x_i - max x) / temperature)
+ *   top-k       the k largest, ties to the lowest index
+ *   top-p       of those the shortest run in falling order (ties: lowest index
+ *               first) whose weights reach top_p of their sum
+ *   min-p       of those the ones with w_i >= min_p
+ *   tokens[r]   the lowest i, in index order, with the kept weights up to and
+ *               including i above u times their sum
+ *   logprobs[r] ln(w_token / that sum); NULL: not wanted.
+ * Weights are formed in 64 bits and summed as integers of 2^-42 or finer (for
+ * a vocabulary of up to 2^20; 2^-44 for 2^18), so neither order nor timing
+ * changes a result. A NaN or -inf logit is never drawn; logits of +inf share
+ * all the weight; a row with nothing to draw gives -1 and -inf. u below 0 or
+ * NaN counts as 0, from 1 as the largest number below it. vocab is at most
+ * 2^20; rows of logits are logits_stride floats apart. Scratch as above. */
+int em_sample(size_t rows, size_t vocab, const float* logits, size_t logits_stride, const float* u,
+              const em_sampling* settings, int* tokens, float* logprobs, void* scratch,
+              void* stream);
+
 /* ---- The device-resident forward pass (cuda_model.h) --------------------- */
 
 /* Replaces struct Config, model.h:11-22: head_size = dim / n_heads,

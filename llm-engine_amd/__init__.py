@@ -33,9 +33,12 @@ EXPORTS = (
     "em_pack_q8", "em_unpack_q8", "em_matmul_q8_packed",
     "em_q8_register", "em_q8_unregister", "em_q8_registered",
     "em_attention_check", "em_attention_scratch_floats", "em_attention",
+    "em_paged_check", "em_paged_append", "em_paged_attention_scratch_floats",
+    "em_paged_attention", "em_sample_scratch_bytes", "em_sample",
     "em_model_create", "em_model_destroy", "em_model_forward",
     "em_model_load", "em_model_config_get", "em_model_read_weight",
 )
+CACHE_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
 ATTN_KERNELS = {"automatic": 0, "single_block": 1, "split": 2}
 
 
@@ -56,6 +59,25 @@ class AttentionShape(ctypes.Structure):
                 ("head_size", ctypes.c_int), ("seq_len", ctypes.c_int),
                 ("q_stride", ctypes.c_size_t), ("kv_stride", ctypes.c_size_t),
                 ("out_stride", ctypes.c_size_t)]
+
+
+class PagedShape(ctypes.Structure):
+    """em_paged_shape."""
+    _fields_ = [(k, ctypes.c_int) for k in ("n_heads", "n_kv_heads", "head_size", "page_size",
+                                            "n_pages", "max_pages", "type")] + \
+               [(k, ctypes.c_size_t) for k in ("page_stride", "slot_stride", "head_stride")]
+
+
+class PagedBatch(ctypes.Structure):
+    """em_paged_batch."""
+    _fields_ = [("n_seqs", ctypes.c_int), ("row_start", ctypes.c_void_p),
+                ("lengths", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_size_t)]
+
+
+class Sampling(ctypes.Structure):
+    """em_sampling."""
+    _fields_ = [(k, ctypes.c_void_p) for k in ("temperature", "top_k", "top_p", "min_p")]
 
 
 class EngineError(Exception):
@@ -141,6 +163,18 @@ def lib() -> ctypes.CDLL:
         L.em_attention_scratch_floats.argtypes = [shp, _sz, ctypes.c_int]
         L.em_attention_scratch_floats.restype = _sz
         L.em_attention.argtypes = [shp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_int, _vp]
+        pshp, pbat = ctypes.POINTER(PagedShape), ctypes.POINTER(PagedBatch)
+        L.em_paged_check.argtypes = [pshp]
+        L.em_paged_append.argtypes = [pshp, pbat, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp,
+                                      ctypes.c_int, ctypes.c_int, _vp, _sz, _vp, _vp, _vp]
+        L.em_paged_attention_scratch_floats.argtypes = [pshp, _sz, _sz]
+        L.em_paged_attention_scratch_floats.restype = _sz
+        L.em_paged_attention.argtypes = [pshp, pbat, _sz, _vp, _sz, _vp, _vp, _vp, _sz,
+                                         ctypes.c_float, ctypes.c_int, _vp, _vp]
+        L.em_sample_scratch_bytes.argtypes = [_sz, _sz]
+        L.em_sample_scratch_bytes.restype = _sz
+        L.em_sample.argtypes = [_sz, _sz, _vp, _sz, _vp, ctypes.POINTER(Sampling), _vp, _vp, _vp,
+                                _vp]
         L.em_model_create.argtypes = [ctypes.POINTER(ModelConfig), _vp,
                                       ctypes.POINTER(LayerWeights), _vp, _vp, ctypes.c_int,
                                       ctypes.POINTER(_vp)]
@@ -418,6 +452,179 @@ def attention(shape: AttentionShape, rows: int, pos_dev, q, key_cache, value_cac
                               _dev(scratch, torch.float32), ATTN_KERNELS.get(kernel, kernel),
                               _stream_ptr(stream)))
     return out
+
+
+# ---- paged KV cache ------------------------------------------------------------
+
+def paged_shape(n_heads, n_kv_heads, head_size, page_size, n_pages, max_pages, dtype="f32",
+                page_stride=None, slot_stride=None, head_stride=None) -> PagedShape:
+    """Caches of [n_pages, page_size, n_kv_heads, head_size] by default; the
+    strides (elements) describe other layouts."""
+    head = head_size if head_stride is None else head_stride
+    slot = n_kv_heads * head_size if slot_stride is None else slot_stride
+    page = page_size * n_kv_heads * head_size if page_stride is None else page_stride
+    return PagedShape(n_heads, n_kv_heads, head_size, page_size, n_pages, max_pages,
+                      CACHE_TYPES.get(dtype, dtype), page, slot, head)
+
+
+def paged_check(shape: PagedShape) -> None:
+    _check(lib().em_paged_check(ctypes.byref(shape)))
+
+
+def _here(stream):
+    """The call's stream, a context that allocates on it, and the current device."""
+    import torch
+    s = stream if stream is not None else torch.cuda.current_stream()
+    device = torch.cuda.current_device()
+    if s.device.index != device:
+        raise InvalidArgument(EM_EINVAL, f"the stream is on {s.device}, the current device is "
+                                         f"cuda:{device}")
+    return s, torch.cuda.stream(s), device
+
+
+def _on(t, what, dtype, device, shape=None):
+    """t's address: of type `dtype`, on the current device, contiguous and of `shape`."""
+    if not t.is_cuda or t.device.index != device or t.dtype != dtype or not t.is_contiguous() or \
+            (shape is not None and tuple(t.shape) != tuple(shape)):
+        of = "" if shape is None else " of shape " + "x".join(map(str, shape))
+        raise InvalidArgument(EM_EINVAL, f"{what}: expected a contiguous {dtype} tensor{of} on "
+                                         f"cuda:{device}")
+    return t.data_ptr()
+
+
+def _rows_of(t, what, rows, width, device):
+    """(address, floats between rows) of a 2-D fp32 tensor of `rows` rows at
+    least `width` wide, its columns together, e.g. a slice of the qkv product's."""
+    import torch
+    if not t.is_cuda or t.device.index != device or t.dtype != torch.float32 or t.dim() != 2 or \
+            t.shape[0] != rows or t.shape[1] < width or (width > 1 and t.stride(1) != 1):
+        raise InvalidArgument(EM_EINVAL, f"{what}: expected {rows} fp32 rows of {width} on "
+                                         f"cuda:{device}")
+    return t.data_ptr(), (t.stride(0) if rows > 1 else max(t.stride(0), width))
+
+
+def _paged_args(shape, row_start, lengths, page_table, key_cache, value_cache, device):
+    import torch
+    _check(lib().em_paged_check(ctypes.byref(shape)))
+    n = lengths.shape[0]
+    if page_table.dim() != 2 or page_table.shape[0] != n or \
+            page_table.shape[1] < shape.max_pages or not page_table.is_cuda or \
+            page_table.device.index != device or page_table.dtype != torch.int32 or \
+            (shape.max_pages > 1 and page_table.stride(1) != 1):
+        raise InvalidArgument(EM_EINVAL, f"page_table: expected {n} int32 rows of "
+                                         f"{shape.max_pages} on cuda:{device}")
+    stride = page_table.stride(0) if n > 1 else max(page_table.stride(0), shape.max_pages)
+    batch = PagedBatch(n, _on(row_start, "row_start", torch.int32, device, (n + 1,)),
+                       _on(lengths, "lengths", torch.int32, device, (n,)), page_table.data_ptr(),
+                       stride)
+    dtype = {0: torch.float32, 1: torch.float16, 2: torch.bfloat16}[shape.type]
+    # One past the last element the shape reaches.
+    last = (shape.n_pages - 1) * shape.page_stride + (shape.page_size - 1) * shape.slot_stride + \
+        (shape.n_kv_heads - 1) * shape.head_stride + shape.head_size
+    for t, what in ((key_cache, "key_cache"), (value_cache, "value_cache")):
+        if not t.is_cuda or t.device.index != device or t.dtype != dtype:
+            raise InvalidArgument(EM_EINVAL, f"{what}: expected {dtype} on cuda:{device}")
+        if 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())) < last:
+            raise InvalidArgument(EM_EINVAL, f"{what}: the shape reaches {last} elements, past "
+                                             "the tensor's last")
+    return batch
+
+
+def paged_append(shape: PagedShape, row_start, lengths, page_table, q, k, v, key_cache,
+                 value_cache, freq=None, halves=False, q_out=None, stream=None):
+    """em_paged_append on torch tensors: q (or None), k and v are 2-D fp32,
+    row-strided views allowed; freq holds rotary / 2 floats (None: no
+    rotation). Returns the rotated queries: q_out (q itself to rotate in
+    place) or a new tensor."""
+    import torch
+    s, ctx, device = _here(stream)
+    batch = _paged_args(shape, row_start, lengths, page_table, key_cache, value_cache, device)
+    rows, dim, kv = k.shape[0], shape.n_heads * shape.head_size, shape.n_kv_heads * shape.head_size
+    qp, qs, op, os_ = None, 0, None, 0
+    if q is not None:
+        qp, qs = _rows_of(q, "q", rows, dim, device)
+        if q_out is None:
+            with ctx:
+                q_out = torch.empty((rows, dim), dtype=torch.float32, device=q.device)
+        op, os_ = _rows_of(q_out, "q_out", rows, dim, device)
+    kp, ks = _rows_of(k, "k", rows, kv, device)
+    vp, vs = _rows_of(v, "v", rows, kv, device)
+    fp, rotary = None, 0
+    if freq is not None and freq.numel():
+        fp, rotary = _on(freq, "freq", torch.float32, device, (freq.numel(),)), 2 * freq.numel()
+    _check(lib().em_paged_append(ctypes.byref(shape), ctypes.byref(batch), rows, qp, qs, kp, ks,
+                                 vp, vs, fp, rotary, int(bool(halves)), op, os_,
+                                 key_cache.data_ptr(), value_cache.data_ptr(),
+                                 int(s.cuda_stream) or None))
+    return q_out
+
+
+def paged_attention_scratch_floats(shape: PagedShape, n_seqs: int, rows: int) -> int:
+    return int(lib().em_paged_attention_scratch_floats(ctypes.byref(shape), n_seqs, rows))
+
+
+def paged_attention(shape: PagedShape, row_start, lengths, page_table, q, key_cache, value_cache,
+                    out=None, scale=0.0, window=0, scratch=None, stream=None):
+    """em_paged_attention on torch tensors: q is 2-D fp32, a row-strided view
+    allowed. A new `out` holds zeros in rows that are no sequence's."""
+    import torch
+    s, ctx, device = _here(stream)
+    batch = _paged_args(shape, row_start, lengths, page_table, key_cache, value_cache, device)
+    rows, dim = q.shape[0], shape.n_heads * shape.head_size
+    qp, qs = _rows_of(q, "q", rows, dim, device)
+    need = paged_attention_scratch_floats(shape, batch.n_seqs, rows)
+    with ctx:
+        if out is None:
+            out = torch.zeros((rows, dim), dtype=torch.float32, device=q.device)
+        if scratch is None:
+            scratch = torch.empty((max(1, need),), dtype=torch.float32, device=q.device)
+    op, os_ = _rows_of(out, "out", rows, dim, device)
+    sp = _on(scratch, "scratch", torch.float32, device)
+    if scratch.numel() < need:
+        raise InvalidArgument(EM_EINVAL, f"scratch: {scratch.numel()} floats, {need} needed")
+    _check(lib().em_paged_attention(ctypes.byref(shape), ctypes.byref(batch), rows, qp, qs,
+                                    key_cache.data_ptr(), value_cache.data_ptr(), op, os_,
+                                    scale, window, sp, int(s.cuda_stream) or None))
+    return out
+
+
+# ---- sampling --------------------------------------------------------------------
+
+def sample_scratch_bytes(rows: int, vocab: int) -> int:
+    return int(lib().em_sample_scratch_bytes(rows, vocab))
+
+
+def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None,
+           logprobs=None, scratch=None, stream=None):
+    """em_sample on torch tensors: logits 2-D fp32 (row-strided views allowed),
+    u and the settings one value a row, top_k int32, the others fp32; None is
+    off (temperature: 1). Returns (tokens int32, logprobs fp32)."""
+    import torch
+    s, ctx, device = _here(stream)
+    if logits.dim() != 2:
+        raise InvalidArgument(EM_EINVAL, "logits: expected 2-D fp32")
+    rows, vocab = logits.shape
+    lp, ls = _rows_of(logits, "logits", rows, vocab, device)
+    opt = lambda t, what, dt: None if t is None else _on(t, what, dt, device, (rows,))
+    settings = Sampling(opt(temperature, "temperature", torch.float32),
+                        opt(top_k, "top_k", torch.int32), opt(top_p, "top_p", torch.float32),
+                        opt(min_p, "min_p", torch.float32))
+    need = sample_scratch_bytes(rows, vocab)
+    with ctx:
+        if tokens is None:
+            tokens = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+        if logprobs is None:
+            logprobs = torch.empty((rows,), dtype=torch.float32, device=logits.device)
+        if scratch is None:
+            scratch = torch.empty((max(1, need),), dtype=torch.uint8, device=logits.device)
+    sp = _on(scratch, "scratch", torch.uint8, device)
+    if scratch.numel() < need:
+        raise InvalidArgument(EM_EINVAL, f"scratch: {scratch.numel()} bytes, {need} needed")
+    _check(lib().em_sample(rows, vocab, lp, ls, _on(u, "u", torch.float32, device, (rows,)),
+                           ctypes.byref(settings), _on(tokens, "tokens", torch.int32, device, (rows,)),
+                           _on(logprobs, "logprobs", torch.float32, device, (rows,)), sp,
+                           int(s.cuda_stream) or None))
+    return tokens, logprobs
 
 
 # ---- the forward pass --------------------------------------------------------
