@@ -280,7 +280,7 @@ typedef struct {
     int n_pages;                        /* pages of each cache */
     int max_pages;                      /* pages of a sequence: columns of the page table */
     int type;                           /* EM_CACHE_* */
-    size_t page_stride, slot_stride, head_stride; /* elements, multiples of 8 */
+    size_t page_stride, slot_stride, head_stride; /* elements, multiples of 8; 2^34 in all */
 } em_paged_shape;
 
 typedef struct {

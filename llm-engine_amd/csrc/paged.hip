@@ -20,17 +20,18 @@ std::string paged_reject(const em_paged_shape& s) {
         return "paged: unknown cache type";
     if (s.page_stride % 8 || s.slot_stride % 8 || s.head_stride % 8)
         return "paged: strides must be multiples of 8";
+    constexpr std::size_t kMaxCache = std::size_t{1} << 34;
     const auto hs = static_cast<std::size_t>(s.head_size);
     if ((s.n_pages > 1 && s.page_stride < hs) || (s.page_size > 1 && s.slot_stride < hs) ||
         (s.n_kv_heads > 1 && s.head_stride < hs))
         return "paged: a stride smaller than head_size";
-    // Every offset below 2^62, so that none overflows on the device.
+    // Offsets in units of eight elements are kept in 32 bits.
     std::size_t a = 0, b = 0, c = 0;
     if (__builtin_mul_overflow(static_cast<std::size_t>(s.n_pages), s.page_stride, &a) ||
         __builtin_mul_overflow(static_cast<std::size_t>(s.page_size), s.slot_stride, &b) ||
         __builtin_mul_overflow(static_cast<std::size_t>(s.n_kv_heads), s.head_stride, &c) ||
-        a >= (std::size_t{1} << 60) || b >= (std::size_t{1} << 60) || c >= (std::size_t{1} << 60))
-        return "paged: caches past 2^60 elements";
+        a >= kMaxCache || b >= kMaxCache || c >= kMaxCache || a + b + c >= kMaxCache)
+        return "paged: caches past 2^34 elements";
     return "";
 }
 

@@ -1,4 +1,18 @@
-// Attention of a batch's rows over a paged KV cache.
+// Attention of a batch's rows over a paged KV cache: new rows of many
+// sequences, one each (a decode step) or chunks of prompts, in one launch and
+// a second that joins what the first split.
+//
+// A sequence's new rows and the heads that share a kv head are its columns:
+// column c is row c / group, head kv head * group + c % group. A work item is
+// (sequence, kv head, 16 columns, run of positions), so a key or value is read
+// once for 16 columns. Both products are MFMAs whose terms keep fp32's
+// accuracy (see Ops); the softmax runs with one pass over the positions, a
+// running maximum and sum in fp32.
+//
+// The lengths are in device memory, so every workgroup forms the plan itself
+// (Plan): the positions of all columns over the workgroups the card holds at
+// once give a run's length, a sequence's positions are cut into runs of about
+// that many, and blockIdx.x is looked up in the running number of items.
 #include <cmath>
 
 #include "paged.hpp"
@@ -6,80 +20,721 @@
 namespace em {
 namespace {
 
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kCols = 16;       // columns of an item
+constexpr int kStep = 32;       // positions a wave takes at a time
+constexpr int kWaves = 4;
+constexpr int kMinRun = 128;    // positions of an item at least: one step a wave
+constexpr uint32_t kNoSlot = 0xffffffffu;
+
 struct PagedAttnArgs {
     PagedArgs p;
     const float* q;
     const void *kc, *vc;
     float* out;
     long long q_stride, out_stride;
-    float scale;
+    float scale2;  // scale times log2 e: weights are 2^(x - max)
     int window;
+    int slots;      // workgroups to spread the positions over
+    float* part_o;  // [unit][16 columns][head_size], a unit an item's 16 columns
+    float2* part_ml;
+    int part_units;
 };
 
-template <class T>
-__device__ __forceinline__ float value_of(T x) {
-    return static_cast<float>(x);
+// --- the plan -----------------------------------------------------------------
+
+// What a sequence asks for, from the batch's arrays.
+struct SeqWork {
+    int row0, n;         // its rows
+    int p0;              // position of the first of them
+    int first, end;      // positions that any row sees
+    int tiles;           // column tiles a kv head
+    __device__ int span() const { return max(1, end - first); }
+};
+
+__device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s) {
+    const PagedArgs& p = a.p;
+    SeqWork w;
+    w.row0 = p.row_start[s];
+    const int r1 = p.row_start[s + 1];
+    w.n = w.row0 >= 0 && r1 <= p.rows && r1 > w.row0 ? r1 - w.row0 : 0;
+    const int len = max(p.lengths[s], -(1 << 29));
+    const int cap = p.page_size * p.max_pages;
+    w.p0 = len - w.n;
+    w.end = min(max(len, 0), cap);
+    w.first = a.window ? min(w.end, max(0, w.p0 + 1 - a.window)) : 0;
+    w.tiles = (w.n * p.group + kCols - 1) / kCols;
+    return w;
 }
 
-// Row blockIdx.x, head blockIdx.y: 256 positions at a time, a score a thread,
-// then a head dim a thread over their values. Positions the row does not see
-// are never read.
-template <class T>
-__global__ __launch_bounds__(kThreads) void paged_row_kernel(PagedAttnArgs a) {
-    const PagedArgs& p = a.p;
-    __shared__ float q_s[256];
-    __shared__ float w_s[kThreads];
-    __shared__ long long off_s[kThreads];
-    __shared__ float part[4];
-    const int r = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, D = p.head_size;
-    const int seq = row_sequence(p, r);
-    if (seq < 0) return;
-    const long long pos = p.lengths[seq] - (static_cast<long long>(p.row_start[seq + 1]) - r);
-    const long long limit = static_cast<long long>(p.max_pages) * p.page_size;
-    const int end = static_cast<int>(max(0LL, min(pos + 1, limit)));
-    const int first = a.window ? static_cast<int>(min(limit, max(0LL, pos + 1 - a.window))) : 0;
-    const T* kc = static_cast<const T*>(a.kc) + (h / p.group) * p.head_stride;
-    const T* vc = static_cast<const T*>(a.vc) + (h / p.group) * p.head_stride;
-    if (tid < D) q_s[tid] = a.q[r * a.q_stride + h * D + tid];
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int t0 = first; t0 < end; t0 += kThreads) {
-        const int t = t0 + tid;
-        const long long off = t < end ? slot_offset(p, seq, t) : -1;
-        __syncthreads();
-        float s = -INFINITY;
-        if (off >= 0) {
-            float dot = 0.0f;
-            for (int d = 0; d < D; ++d) dot = fmaf(q_s[d], value_of(kc[off + d]), dot);
-            s = dot * a.scale;
+__device__ __forceinline__ int wave_sum_int(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+    return v;
+}
+__device__ __forceinline__ int wave_scan_int(int v) {  // inclusive
+    const int lane = threadIdx.x % kWave;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const int o = __shfl_up(v, d, kWave);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+// A run's positions: all columns' positions over the slots.
+__device__ __forceinline__ float run_length(const PagedAttnArgs& a) {
+    const int lane = threadIdx.x % kWave;
+    float total = 0.0f;
+    for (int s0 = 0; s0 < a.p.n_seqs; s0 += kWave) {
+        float t = 0.0f;
+        if (s0 + lane < a.p.n_seqs) {
+            const SeqWork w = seq_work(a, s0 + lane);
+            t = static_cast<float>(w.tiles) * static_cast<float>(w.span());
         }
-        const float mn = fmaxf(m, block_max(s, part));
-        const float alpha = mn == -INFINITY ? 1.0f : expf(m - mn);
-        const float w = off < 0 || s == -INFINITY ? 0.0f : expf(s - mn);
-        off_s[tid] = off;
-        w_s[tid] = w;
-        l = l * alpha + block_sum(w, part);  // its barriers publish the weights
-        m = mn;
-        o *= alpha;
-        if (tid < D) {
-            const int n = min(kThreads, end - t0);
-            for (int i = 0; i < n; ++i)
-                if (off_s[i] >= 0) o = fmaf(w_s[i], value_of(vc[off_s[i] + tid]), o);
+        total += wave_sum(t);
+    }
+    total *= static_cast<float>(a.p.n_kv_heads);
+    return fmaxf(static_cast<float>(kMinRun), total / static_cast<float>(a.slots));
+}
+
+// Runs of a sequence: its positions over a run's length, rounded to nearest,
+// so that no item is longer than one and a half of them.
+__device__ __forceinline__ int runs_of(const SeqWork& w, float run) {
+    return max(1, min(1 << 16, static_cast<int>(static_cast<float>(w.span()) / run + 0.5f)));
+}
+
+// Finds by wave the sequence for which `hit(s, items before, items of it)`
+// holds, walking the running sums; `units` counts the partials' units
+// likewise (sequences of one run need none, and none is split past the
+// partials' memory).
+struct Found {
+    int seq, runs, item0, unit0;
+    SeqWork w;
+};
+template <class Hit>
+__device__ __forceinline__ bool find(const PagedAttnArgs& a, float run, Hit hit, Found& f) {
+    const int lane = threadIdx.x % kWave;
+    int items = 0, units = 0;
+    for (int s0 = 0; s0 < a.p.n_seqs; s0 += kWave) {
+        const int s = s0 + lane;
+        SeqWork w{};
+        int cells = 0, runs = 0;
+        if (s < a.p.n_seqs) {
+            w = seq_work(a, s);
+            cells = w.tiles * a.p.n_kv_heads;
+            runs = runs_of(w, run);
+        }
+        // Units by the runs wanted; a sequence that would pass the partials'
+        // memory stays whole (its units stay counted: all after it do too).
+        const int want = runs > 1 ? cells * runs : 0;
+        const int ahead = units + wave_scan_int(want) - want;
+        if (ahead + want > a.part_units) runs = min(runs, 1);
+        const int mine = cells * runs;
+        const int before = items + wave_scan_int(mine) - mine;
+        const unsigned long long got = __ballot(s < a.p.n_seqs && hit(s, before, mine));
+        if (got) {
+            const int src = __ffsll(got) - 1;
+            f.seq = s0 + src;
+            f.runs = __shfl(runs, src, kWave);
+            f.item0 = __shfl(before, src, kWave);
+            f.unit0 = __shfl(ahead, src, kWave);
+            f.w.row0 = __shfl(w.row0, src, kWave);
+            f.w.n = __shfl(w.n, src, kWave);
+            f.w.p0 = __shfl(w.p0, src, kWave);
+            f.w.first = __shfl(w.first, src, kWave);
+            f.w.end = __shfl(w.end, src, kWave);
+            f.w.tiles = __shfl(w.tiles, src, kWave);
+            return true;
+        }
+        items = __shfl(before + mine, kWave - 1, kWave);
+        units = __shfl(ahead + want, kWave - 1, kWave);
+    }
+    return false;
+}
+
+// --- types ----------------------------------------------------------------------
+
+// The MFMA terms of each cache type. Queries and weights are fp32, so each is
+// held as a sum of 16-bit terms and the products are added in fp32:
+//   bf16 caches: three bf16 terms, exact down to 2^-109, times the value as it
+//     is: three products.
+//   fp32 caches: both sides three bf16 terms; the three products of the
+//     smallest (below 2^-24 of the whole) are left out: six products.
+//   fp16 caches: two fp16 terms of a column scaled to a largest query value
+//     of 2^14 (weights: 2^14 for 1), off by 2^-22 of the value and 2^-39 of the
+//     largest; fp16 keys and values are at most 2^16: two products.
+template <class T>
+struct Ops;
+
+template <>
+struct Ops<__bf16> {
+    using Frag = bf16x8;
+    static constexpr int kTerms = 3, kCacheTerms = 1;
+    static constexpr float kWeight = 1.0f;
+};
+template <>
+struct Ops<float> {
+    using Frag = bf16x8;
+    static constexpr int kTerms = 3, kCacheTerms = 3;
+    static constexpr float kWeight = 1.0f;
+};
+template <>
+struct Ops<_Float16> {
+    using Frag = f16x8;
+    static constexpr int kTerms = 2, kCacheTerms = 1;
+    static constexpr float kWeight = 16384.0f;
+};
+
+__device__ __forceinline__ floatx4 mma16(f16x8 a, f16x8 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx4 mma16(bf16x8 a, bf16x8 b, floatx4 c) {
+    return mfma16x16x32(a, b, c);
+}
+
+// Eight fp32 values as terms. lost: as split3x8's (bf16).
+__device__ __forceinline__ void split_terms(const float (&v)[8], bf16x8 (&t)[3], uint32_t& lost) {
+    uint4 x[3];
+    split3x8(v, x, lost);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) t[i] = __builtin_bit_cast(bf16x8, x[i]);
+}
+__device__ __forceinline__ void split_terms(const float (&v)[8], f16x8 (&t)[2], uint32_t&) {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        t[0][e] = static_cast<_Float16>(v[e]);
+        t[1][e] = static_cast<_Float16>(v[e] - static_cast<float>(t[0][e]));
+    }
+}
+
+// 16-bit caches are loaded as they are (four dwords for eight values), fp32 as
+// two vectors.
+template <class T>
+struct Raw8 {
+    uint4 x;
+    __device__ void load(const T* p) { x = *reinterpret_cast<const uint4*>(p); }
+    __device__ void zero() { x = make_uint4(0, 0, 0, 0); }
+};
+template <>
+struct Raw8<float> {
+    float v[8];
+    __device__ void load(const float* p) {
+        const floatx4 a = *reinterpret_cast<const floatx4*>(p);
+        const floatx4 b = *reinterpret_cast<const floatx4*>(p + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = a[i];
+            v[4 + i] = b[i];
         }
     }
-    if (tid < D) a.out[r * a.out_stride + h * D + tid] = l == 0.0f ? 0.0f : o / l;
+    __device__ void zero() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    }
+};
+
+__device__ __forceinline__ uint32_t word(const uint4& x, int i) {
+    return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w;
 }
 
-void run_paged_attention(const PagedAttnArgs& a, int type, hipStream_t stream) {
-    const dim3 grid(a.p.rows, a.p.n_heads), block(kThreads);
-    if (type == EM_CACHE_F32)
-        hipLaunchKernelGGL(paged_row_kernel<float>, grid, block, 0, stream, a);
-    else if (type == EM_CACHE_F16)
-        hipLaunchKernelGGL(paged_row_kernel<_Float16>, grid, block, 0, stream, a);
+// d += A x B over the pairs of terms kept.
+template <class F, int NT>
+__device__ __forceinline__ void mma_terms(const F (&k)[1], const F (&q)[NT], floatx4& d) {
+#pragma unroll
+    for (int t = NT - 1; t >= 0; --t) d = mma16(k[0], q[t], d);
+}
+template <class F>
+__device__ __forceinline__ void mma_terms(const F (&k)[3], const F (&q)[3], floatx4& d) {
+    d = mma16(k[2], q[0], d);
+    d = mma16(k[1], q[1], d);
+    d = mma16(k[0], q[2], d);
+    d = mma16(k[1], q[0], d);
+    d = mma16(k[0], q[1], d);
+    d = mma16(k[0], q[0], d);
+}
+
+// --- one column, plainly ------------------------------------------------------------
+
+// The slot of position t in units of eight elements, or kNoSlot.
+__device__ __forceinline__ uint32_t slot_unit(const PagedArgs& p, int seq, int t) {
+    const long long off = slot_offset(p, seq, t);
+    return off < 0 ? kNoSlot : static_cast<uint32_t>(off >> 3);
+}
+
+// One wave, one column over positions lo, lo + 1 .. of every stride-th run of
+// 32 before hi, in fp32 operations on what the column sees alone: for columns
+// whose operands the terms do not hold, and for those beside a position that
+// is not finite and that they do not see (its zero weight would not hide it).
+// m, l: maximum (of log2 weights) and sum; o[i]: head dim lane + 64 i,
+// unnormalised.
+template <class T, int N>
+__device__ __noinline__ void plain_column(const PagedAttnArgs& a, int seq, int row, int head,
+                                          int pq, int lo, int hi, int stride, float& m, float& l,
+                                          float (&o)[N]) {
+    const PagedArgs& p = a.p;
+    const int lane = threadIdx.x % kWave, D = p.head_size;
+    const float* q = a.q + row * a.q_stride + head * D;
+    const long long hoff = (head / p.group) * p.head_stride;
+    const T* kc = static_cast<const T*>(a.kc) + hoff;
+    const T* vc = static_cast<const T*>(a.vc) + hoff;
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = 0.0f;
+    for (int t0 = lo; t0 < hi; t0 += stride) {
+        const int t = t0 + lane;
+        uint32_t unit = kNoSlot;
+        if (lane < kStep && t < hi && t <= pq && !(a.window && t <= pq - a.window))
+            unit = slot_unit(p, seq, t);
+        float x = -INFINITY;
+        if (unit != kNoSlot) {
+            const T* k = kc + static_cast<std::size_t>(unit) * 8;
+            float dot = 0.0f;
+            for (int d = 0; d < D; ++d) dot = fmaf(q[d], static_cast<float>(k[d]), dot);
+            x = dot * a.scale2;
+        }
+        const float mn = fmaxf(m, wave_max(x));
+        const float alpha = mn == -INFINITY ? 1.0f : exp2f(m - mn);
+        const float w = unit == kNoSlot || x == -INFINITY ? 0.0f : exp2f(x - mn);
+        m = mn;
+        l = l * alpha + wave_sum(w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] *= alpha;
+        for (int i = 0; i < kStep; ++i) {
+            const uint32_t u = __shfl(unit, i, kWave);
+            if (u == kNoSlot) continue;
+            const float wi = __shfl(w, i, kWave);
+            const T* v = vc + static_cast<std::size_t>(u) * 8;
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                if (lane + kWave * n < D)
+                    o[n] = fmaf(wi, static_cast<float>(v[lane + kWave * n]), o[n]);
+        }
+    }
+}
+
+// --- 16 columns ---------------------------------------------------------------------
+
+// An item: 16 columns over positions [lo, hi), its four waves taking every
+// fourth 32 of them. In lane (g, j) of a wave, per 32 positions:
+//  * S^T = K Q^T: position j (16 + j) of the first operand, head dims 8g .. of
+//    each 32, loaded from the cache as the MFMA takes them; Q's terms stay in
+//    registers.
+//  * The lane ends with column j's scores at positions 4g + r and 16 + 4g + r:
+//    its eight k values of O^T += V^T P^T once V's operand takes positions in
+//    that order.
+//  * V: a lane loads VU head dims VU j .. of its eight positions, 256 bytes of
+//    a position by 16 lanes, and eight-position columns of them are put
+//    together by byte permutes (fp32: by the split).
+//  * O^T: column j, head dims VU (4g + r) + u.
+// Nothing is staged in LDS: 16 KB a wave are in flight (keys are loaded again
+// right after their product, values after theirs), which 8 waves a CU need to
+// keep HBM busy.
+template <class T, int DP>
+struct Few {
+    static constexpr int C = DP / 32, VU = DP / 16, NV = (VU + 7) / 8;
+    using O = Ops<T>;
+    using Frag = typename O::Frag;
+    static constexpr int NT = O::kTerms, KT = O::kCacheTerms;
+};
+
+// A 16-bit value operand: element u of eight positions.
+template <class F, class T, int NV>
+__device__ __forceinline__ void value_terms(const Raw8<T> (&v)[8][NV], int u, F (&t)[1], uint32_t&) {
+    const uint32_t sel = u & 1 ? 0x07060302u : 0x05040100u;
+    const int n = u / 8, wd = (u % 8) / 2;
+    uint4 x;
+    x.x = __builtin_amdgcn_perm(word(v[1][n].x, wd), word(v[0][n].x, wd), sel);
+    x.y = __builtin_amdgcn_perm(word(v[3][n].x, wd), word(v[2][n].x, wd), sel);
+    x.z = __builtin_amdgcn_perm(word(v[5][n].x, wd), word(v[4][n].x, wd), sel);
+    x.w = __builtin_amdgcn_perm(word(v[7][n].x, wd), word(v[6][n].x, wd), sel);
+    t[0] = __builtin_bit_cast(F, x);
+}
+template <class F, int NV>
+__device__ __forceinline__ void value_terms(const Raw8<float> (&v)[8][NV], int u, F (&t)[3],
+                                            uint32_t& lost) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = v[e][u / 8].v[u % 8];
+    split_terms(x, t, lost);
+}
+template <class F, class T>
+__device__ __forceinline__ void key_terms(const Raw8<T>& k, F (&t)[1]) {
+    t[0] = __builtin_bit_cast(F, k.x);
+}
+template <class F>
+__device__ __forceinline__ void key_terms(const Raw8<float>& k, F (&t)[3]) {
+    uint32_t lost = 0;  // a query too large for it to matter is found with the query
+    split_terms(k.v, t, lost);
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_few_kernel(PagedAttnArgs a) {
+    using F = Few<T, DP>;
+    constexpr int C = F::C, VU = F::VU, NV = F::NV, NT = F::NT, KT = F::KT;
+    constexpr int kRow = DP + 4;  // floats of a column in LDS
+    __shared__ __attribute__((aligned(16))) float o_s[kWaves][kCols][kRow];
+    __shared__ float2 ml_s[kWaves][kCols];
+    const PagedArgs& p = a.p;
+    const int tid = threadIdx.x, lane = tid % kWave, g = lane >> 4, j = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int D = p.head_size, item = blockIdx.x;
+
+    Found f;
+    const float run = run_length(a);
+    if (!find(a, run, [&](int, int before, int mine) { return item >= before && item < before + mine; },
+              f))
+        return;
+    // Item order in a sequence: kv heads fastest (the XCDs take blocks in
+    // turn, so a kv head's tiles share an L2), the longest tiles first.
+    const int at = item - f.item0, kvh = at % p.n_kv_heads;
+    const int tile = f.w.tiles - 1 - at / p.n_kv_heads % f.w.tiles;
+    const int part = at / p.n_kv_heads / f.w.tiles;
+    const int cols = min(kCols, f.w.n * p.group - tile * kCols);
+    const int col = tile * kCols + min(j, cols - 1);
+    const int i = col / p.group, row = f.w.row0 + i, head = kvh * p.group + col % p.group;
+    const int pq = f.w.p0 + i;
+    // The tile's positions, this item's run of them.
+    const int i0 = tile * kCols / p.group, i1 = (tile * kCols + cols - 1) / p.group;
+    const int first = max(f.w.first, a.window ? f.w.p0 + i0 + 1 - a.window : 0);
+    const int end = min(f.w.end, f.w.p0 + i1 + 1);
+    const int len = ((max(0, end - first) + f.runs - 1) / f.runs + kStep - 1) / kStep * kStep;
+    const int lo = first + part * len, hi = min(end, lo + len);
+    // Every column sees positions [all_lo, all_hi].
+    const int all_lo = a.window ? f.w.p0 + i1 + 1 - a.window : 0, all_hi = f.w.p0 + i0;
+
+    // The column's query terms.
+    typename F::Frag q[C][NT];
+    uint32_t lost_q = 0, lost_v = 0;
+    float top_q = 0.0f, unscale = 1.0f;
+    {
+        float v[C][8];
+        const float* src = a.q + row * a.q_stride + head * D;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int d = 32 * c + 8 * g;
+            const bool in = d < D;
+            const floatx4 x0 = *reinterpret_cast<const floatx4*>(src + (in ? d : 0));
+            const floatx4 x1 = *reinterpret_cast<const floatx4*>(src + (in ? d : 0) + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[c][e] = in ? x0[e] * a.scale2 : 0.0f;
+                v[c][4 + e] = in ? x1[e] * a.scale2 : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top_q = fmaxf(top_q, fabsf(v[c][e]));
+        }
+        top_q = max32(max16(top_q));
+        if constexpr (NT == 2) {
+            // To a largest value of 2^14 .. 2^15.
+            const int ex = top_q > 0.0f && top_q < INFINITY ? 14 - ilogbf(top_q) : 0;
+            const float up = ldexpf(1.0f, min(ex, 120));
+            unscale = ldexpf(1.0f, -min(ex, 120));
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[c][e] *= up;
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) split_terms(v[c], q[c], lost_q);
+    }
+    // fp32 keys below 2^-109 drop bits worth up to 2^-134 each: nothing for a
+    // query below 2^90. fp16's scale reaches down to 2^-106.
+    bool bad = KT == 3   ? (lost_q & 0xffffu) != 0 || !(top_q < 0x1p90f)
+               : NT == 3 ? (lost_q & 0xffffu) != 0
+                         : top_q != 0.0f && !(top_q >= 0x1p-100f && top_q < INFINITY);
+
+    const T* kc = static_cast<const T*>(a.kc) + kvh * p.head_stride;
+    const T* vc = static_cast<const T*>(a.vc) + kvh * p.head_stride;
+    // Lane l holds position l % 32 of a step. Positions that are not there
+    // read slot 0 and count for nothing.
+    auto units = [&](int t0) {
+        const int t = t0 + (lane & 31);
+        return t < hi ? slot_unit(p, f.seq, t) : kNoSlot;
+    };
+    Raw8<T> k[2][C], v[8][NV];
+    auto load_k = [&](uint32_t u) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const uint32_t x = __shfl(u, 16 * y + j, kWave);
+            const T* src = kc + static_cast<std::size_t>(x == kNoSlot ? 0 : x) * 8;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const int d = 32 * c + 8 * g;
+                k[y][c].load(src + (d < D ? d : 0));
+            }
+        }
+    };
+    auto load_v = [&](uint32_t u) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t x = __shfl(u, 4 * g + (e < 4 ? e : 12 + e), kWave);
+            const T* src = vc + static_cast<std::size_t>(x == kNoSlot ? 0 : x) * 8;
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const int d = VU * j + 8 * n;
+                if constexpr (VU == 4) {
+                    // Four head dims a lane: half a vector.
+                    const T* s4 = src + (d < D ? d : 0);
+                    if constexpr (sizeof(T) == 4) {
+                        const floatx4 y = *reinterpret_cast<const floatx4*>(s4);
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) v[e][n].v[z] = y[z];
+                    } else {
+                        const uint2 y = *reinterpret_cast<const uint2*>(s4);
+                        v[e][n].x = make_uint4(y.x, y.y, 0, 0);
+                    }
+                } else {
+                    v[e][n].load(src + (d < D ? d : 0));
+                }
+            }
+        }
+    };
+
+    float m = -INFINITY, l = 0.0f;
+    floatx4 o[VU];
+#pragma unroll
+    for (int u = 0; u < VU; ++u) o[u] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+    constexpr int kStride = kStep * kWaves;
+    int t0 = lo + w * kStep;
+    if (t0 < hi) {
+        uint32_t u = units(t0);
+        load_k(u);
+        load_v(u);
+        while (true) {
+            const uint32_t un = units(t0 + kStride);
+            floatx4 s[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                s[y] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    typename F::Frag kt[KT];
+                    key_terms(k[y][c], kt);
+                    mma_terms(kt, q[c], s[y]);
+                }
+            }
+            const bool more = t0 + kStride < hi;
+            if (more) load_k(un);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = NT == 2 ? s[e / 4][e % 4] * unscale : s[e / 4][e % 4];
+            // Positions that are there, of the step's 32.
+            const uint32_t there = static_cast<uint32_t>(__ballot(u != kNoSlot));
+            if (there != 0xffffffffu || t0 < all_lo || t0 + kStep - 1 > all_hi) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int r = 4 * g + (e < 4 ? e : 12 + e), t = t0 + r;
+                    const bool seen =
+                        (there >> r & 1) && t <= pq && !(a.window && t <= pq - a.window);
+                    x[e] = seen ? x[e] : -INFINITY;
+                }
+                if (there != 0xffffffffu) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (!(there >> (4 * g + (e < 4 ? e : 12 + e)) & 1)) {
+#pragma unroll
+                            for (int n = 0; n < NV; ++n) v[e][n].zero();
+                        }
+                }
+            }
+            float mb = x[0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) mb = fmaxf(mb, x[e]);
+            const float mn = fmaxf(m, max32(max16(mb)));
+            if (__ballot(mn > m)) {
+                const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+                l *= alpha;
+#pragma unroll
+                for (int y = 0; y < VU; ++y) o[y] *= alpha;
+                m = mn;
+            }
+            const float base = mn == -INFINITY ? 0.0f : mn;
+            float pw[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                pw[e] = __builtin_amdgcn_exp2f(x[e] - base);
+                l += pw[e];
+                pw[e] *= F::O::kWeight;
+            }
+            typename F::Frag pt[NT];
+            uint32_t lost_p = 0;
+            split_terms(pw, pt, lost_p);
+#pragma unroll
+            for (int y = 0; y < VU; ++y) {
+                typename F::Frag vt[KT];
+                value_terms(v, y, vt, lost_v);
+                mma_terms(vt, pt, o[y]);
+            }
+            if (!more) break;
+            load_v(un);
+            u = un;
+            t0 += kStride;
+        }
+    }
+    l = sum32(sum16(l));
+    float low = INFINITY;
+#pragma unroll
+    for (int y = 0; y < VU; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int d = VU * (4 * g + r) + y;
+            const float x = fabsf(o[y][r]);
+            bad |= d < D && !(x < INFINITY);
+            low = d < D ? fminf(low, x) : low;
+        }
+    // fp32 values that dropped bits, worth up to 2^-134 each, beside a sum so
+    // small that it could show.
+    if constexpr (KT == 3) bad |= __ballot((lost_v & 0xffffu) != 0) != 0 && low < 0x1p-50f;
+    bad |= !(l < INFINITY);
+    // A column's lanes together.
+    unsigned long long redo = __ballot(bad);
+    redo |= redo >> 32;
+    redo = (redo | redo >> 16) & 0xffffu;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int y = 0; y < VU; ++y)
+            o_s[w][j][VU * (4 * g + r) + y] = o[y][r] * (1.0f / F::O::kWeight);
+    if (g == 0) ml_s[w][j] = make_float2(m, l);
+    while (redo) {
+        const int c = __ffsll(redo) - 1;
+        redo &= redo - 1;
+        float po[DP / kWave], pm, pl;
+        plain_column<T, DP / kWave>(a, f.seq, __shfl(row, c, kWave), __shfl(head, c, kWave),
+                                    __shfl(pq, c, kWave), lo + w * kStep, hi, kStride, pm, pl, po);
+#pragma unroll
+        for (int n = 0; n < DP / kWave; ++n) o_s[w][c][lane + kWave * n] = po[n];
+        if (lane == 0) ml_s[w][c] = make_float2(pm, pl);
+    }
+    __syncthreads();
+
+    // The four waves' sums, in wave order.
+    const int unit = f.unit0 + at;
+    for (int x = tid; x < cols * (D / 4); x += kThreads) {
+        const int c = x / (D / 4), d = x % (D / 4) * 4;
+        float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+        for (int y = 0; y < kWaves; ++y) mm = fmaxf(mm, ml_s[y][c].x);
+        floatx4 sum{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int y = 0; y < kWaves; ++y) {
+            const float2 ml = ml_s[y][c];
+            // A wave whose sum is NaN has no maximum to go by.
+            const float fac = ml.x == mm || ml.y != ml.y ? 1.0f
+                              : ml.x == -INFINITY        ? 0.0f
+                                                         : __builtin_amdgcn_exp2f(ml.x - mm);
+            ll += fac * ml.y;
+            sum += fac * *reinterpret_cast<const floatx4*>(&o_s[y][c][d]);
+        }
+        const int cc = tile * kCols + c;
+        if (f.runs > 1) {
+            const std::size_t pc = static_cast<std::size_t>(unit) * kCols + c;
+            *reinterpret_cast<floatx4*>(a.part_o + pc * D + d) = sum;
+            if (d == 0) a.part_ml[pc] = make_float2(mm, ll);
+        } else {
+            float* dst = a.out + (f.w.row0 + cc / p.group) * a.out_stride +
+                         (kvh * p.group + cc % p.group) * D + d;
+            *reinterpret_cast<floatx4*>(dst) = ll == 0.0f ? floatx4{0.f, 0.f, 0.f, 0.f} : sum * (1.0f / ll);
+        }
+    }
+}
+
+// Joins the runs of a sequence that was split: row blockIdx.x, kv head
+// blockIdx.y, a thread four head dims of a column, the runs in order.
+__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a) {
+    const PagedArgs& p = a.p;
+    const int r = blockIdx.x, kvh = blockIdx.y, D = p.head_size;
+    const int seq = row_sequence(p, r);
+    if (seq < 0) return;
+    Found f;
+    const float run = run_length(a);
+    if (!find(a, run, [&](int s, int, int) { return s == seq; }, f) || f.runs <= 1) return;
+    for (int x = threadIdx.x; x < p.group * (D / 4); x += kThreads) {
+        const int h = x / (D / 4), d = x % (D / 4) * 4;
+        const int cc = (r - f.w.row0) * p.group + h, tile = cc / kCols, c = cc % kCols;
+        const int step = f.w.tiles * p.n_kv_heads;
+        const std::size_t u0 = f.unit0 + (f.w.tiles - 1 - tile) * p.n_kv_heads + kvh;
+        float m = -INFINITY;
+        for (int y = 0; y < f.runs; ++y)
+            m = fmaxf(m, a.part_ml[(u0 + static_cast<std::size_t>(y) * step) * kCols + c].x);
+        float l = 0.0f;
+        floatx4 sum{0.f, 0.f, 0.f, 0.f};
+        for (int y = 0; y < f.runs; ++y) {
+            const std::size_t pc = (u0 + static_cast<std::size_t>(y) * step) * kCols + c;
+            const float2 ml = a.part_ml[pc];
+            const float fac = ml.x == m || ml.y != ml.y ? 1.0f
+                              : ml.x == -INFINITY       ? 0.0f
+                                                        : __builtin_amdgcn_exp2f(ml.x - m);
+            l += fac * ml.y;
+            sum += fac * *reinterpret_cast<const floatx4*>(a.part_o + pc * D + d);
+        }
+        float* dst = a.out + r * a.out_stride + (kvh * p.group + h) * D + d;
+        *reinterpret_cast<floatx4*>(dst) = l == 0.0f ? floatx4{0.f, 0.f, 0.f, 0.f} : sum * (1.0f / l);
+    }
+}
+
+// --- launch ---------------------------------------------------------------------------
+
+int paged_slots() { return 2 * cu_count(); }
+
+// Whether any sequence of the shape can be split: it needs one and a half
+// runs' positions.
+bool can_split(const em_paged_shape& s) {
+    return static_cast<long long>(s.page_size) * s.max_pages >= kMinRun * 3 / 2;
+}
+
+// Units of partials at most. A sequence of two runs or more has them over 1.5
+// lengths or more, so runs <= 4/3 positions / length, and all columns'
+// positions / length is at most the slots; one sixteenth is added for the
+// float arithmetic of the plan.
+int partial_units(const em_paged_shape& s) {
+    return can_split(s) ? paged_slots() * 17 / 12 + 1 : 0;
+}
+
+std::size_t paged_attention_scratch(const em_paged_shape& s, std::size_t, std::size_t) {
+    return static_cast<std::size_t>(partial_units(s)) * kCols *
+           (static_cast<std::size_t>(s.head_size) + 2);
+}
+
+template <class T>
+void launch_few(const PagedAttnArgs& a, dim3 grid, hipStream_t stream) {
+    if (a.p.head_size <= 64)
+        hipLaunchKernelGGL((paged_few_kernel<T, 64>), grid, dim3(kThreads), 0, stream, a);
+    else if (a.p.head_size <= 128)
+        hipLaunchKernelGGL((paged_few_kernel<T, 128>), grid, dim3(kThreads), 0, stream, a);
     else
-        hipLaunchKernelGGL(paged_row_kernel<__bf16>, grid, block, 0, stream, a);
+        hipLaunchKernelGGL((paged_few_kernel<T, 256>), grid, dim3(kThreads), 0, stream, a);
 }
 
-std::size_t paged_attention_scratch(const em_paged_shape&, std::size_t, std::size_t) { return 0; }
+void run_paged_attention(PagedAttnArgs a, const em_paged_shape& s, float* scratch,
+                         hipStream_t stream) {
+    a.slots = paged_slots();
+    a.part_units = partial_units(s);
+    a.part_o = scratch;
+    a.part_ml = reinterpret_cast<float2*>(
+        scratch + static_cast<std::size_t>(a.part_units) * kCols * s.head_size);
+    // Column tiles at most (each sequence's last may be partly full), a run
+    // more for each run length in all columns' positions.
+    const long long cols = static_cast<long long>(a.p.rows) * a.p.group;
+    const long long tiles = cols / kCols + std::min(a.p.n_seqs, a.p.rows);
+    const long long items = tiles * a.p.n_kv_heads + (a.part_units ? a.slots + a.slots / 16 + 1 : 0);
+    const dim3 grid(static_cast<unsigned>(items));
+    if (s.type == EM_CACHE_F32)
+        launch_few<float>(a, grid, stream);
+    else if (s.type == EM_CACHE_F16)
+        launch_few<_Float16>(a, grid, stream);
+    else
+        launch_few<__bf16>(a, grid, stream);
+    if (a.part_units)
+        hipLaunchKernelGGL(paged_join_kernel, dim3(a.p.rows, a.p.n_kv_heads), dim3(kThreads), 0,
+                           stream, a);
+}
 
 bool a16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -105,7 +760,8 @@ int em_paged_attention(const em_paged_shape* s, const em_paged_batch* b, size_t 
     if (!b) return fail(EM_EINVAL, "paged_attention: null batch");
     const std::string why = em::paged_batch_reject(*s, *b, rows);
     if (!why.empty()) return fail(EM_EINVAL, why);
-    if (window < 0) return fail(EM_EINVAL, "paged_attention: negative window");
+    if (window < 0 || window > (1 << 30))
+        return fail(EM_EINVAL, "paged_attention: a window of 0 to 2^30 positions");
     if (!std::isfinite(scale)) return fail(EM_EINVAL, "paged_attention: scale is not finite");
     if (rows == 0 || b->n_seqs == 0) return EM_OK;
     const size_t need =
@@ -131,10 +787,10 @@ int em_paged_attention(const em_paged_shape* s, const em_paged_batch* b, size_t 
         a.out = out;
         a.q_stride = static_cast<long long>(q_stride);
         a.out_stride = static_cast<long long>(out_stride);
-        a.scale = scale != 0.0f ? scale
-                                : static_cast<float>(1.0 / std::sqrt(static_cast<double>(s->head_size)));
+        const double by = scale != 0.0f ? scale : 1.0 / std::sqrt(static_cast<double>(s->head_size));
+        a.scale2 = static_cast<float>(by * 1.4426950408889634074);
         a.window = window;
-        em::run_paged_attention(a, s->type, static_cast<hipStream_t>(stream));
+        em::run_paged_attention(a, *s, scratch, static_cast<hipStream_t>(stream));
         em::hip_check(hipGetLastError(), "launch");
     } catch (const std::exception& e) {
         return fail(EM_EDEVICE, e.what());

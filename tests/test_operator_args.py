@@ -56,7 +56,7 @@ BAD_SHAPES = [
     (dict(page_size=1 << 16, max_pages=1 << 15), "2^30 positions"),
     (dict(dtype=7), "cache type"), (dict(slot_stride=132), "multiples of 8"),
     (dict(head_stride=56), "smaller than head_size"), (dict(slot_stride=0), "smaller"),
-    (dict(page_stride=0), "smaller"), (dict(page_stride=1 << 58), "2^60"),
+    (dict(page_stride=0), "smaller"), (dict(page_stride=1 << 58), "2^34"),
 ]
 
 
@@ -97,7 +97,7 @@ def test_append_arguments():
 
 
 def test_attention_arguments():
-    for kw, why in ((dict(window=-1), "window"), (dict(scale=float("inf")), "scale"),
+    for kw, why in ((dict(window=-1), "window"), (dict(window=(1 << 30) + 1), "window"), (dict(scale=float("inf")), "scale"),
                     (dict(scale=float("nan")), "scale"), (dict(q=None), "null"),
                     (dict(kc=None), "null"), (dict(vc=None), "null"), (dict(out=None), "null"),
                     (dict(qs=500), "strides"), (dict(os_=514), "strides"), (dict(q=P + 4), "aligned"),
