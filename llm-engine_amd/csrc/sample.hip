@@ -1,17 +1,23 @@
 // Sampling: the next token of each row of logits by temperature, top-k,
 // top-p and min-p from a given uniform number.
 //
-// A token's weight w = exp((x - max) / T) is formed in 64 bits and summed as
-// an integer, round(w 2^bits), bits = 62 - ceil(log2 vocab): the row's sum
-// stays below 2^63, sums do not depend on the order they are formed in, and
-// which side of a border u falls on is off by 2^-43 of a vocabulary's largest
-// weight and less, where fp32 sums of 100000 weights lose 2^-20 of it.
+// A token's weight w = exp((x - max) / T) is formed in 64 bits, so that which
+// side of a border u falls on is off by some 2^-50 of the sum, where fp32 sums
+// of 100000 weights lose 2^-20 of it. Where weights are added by atomics, in an
+// order that changes, they are integers, round(w 2^bits) with bits = 62 -
+// ceil(log2 vocab): the row's sum stays below 2^63 and is always the same.
 //
-// Both filters are thresholds on the logit: top-k's and top-p's last token
-// kept is a value and a number of tokens of just that value, lowest index
-// first, found by radix selection on the logits' ordered bits (top-k by
-// counts, top-p by summed weights). The draw then adds the kept weights in
-// index order.
+// Both filters are thresholds on the logit: the last token kept is a value and
+// a number of tokens of just that value, lowest index first. A histogram over
+// the distance from the maximum (counts for top-k, weights for top-p) names the
+// bin it lies in, and the few tokens of that bin are ranked against each other;
+// a bin with too many (ties, or a maximum far above the rest) is resolved by
+// radix selection on the logits' bits instead. The draw then adds the kept
+// weights in index order: a total per wave, whose run of the row the whole
+// workgroup then goes through.
+//
+// One workgroup a row, 16 waves each with its own run of consecutive logits;
+// rows of up to 32765 are read once, into LDS, longer ones once a pass.
 #include <cmath>
 
 #include "internal.hpp"
@@ -23,9 +29,10 @@ namespace {
 using u64 = unsigned long long;
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWaves = kSampleThreads / kWave;
-constexpr int kSegment = 256;                 // values a wave takes at once
+constexpr int kChunk = 4 * kWave;  // logits a wave reads at once
 constexpr int kMaxVocab = 1 << 20;
-constexpr int kMaxSegments = kMaxVocab / kSegment;
+constexpr int kBins = 2048;
+constexpr int kList = 512;  // tokens of a bin that are ranked against each other
 
 struct SampleArgs {
     int rows, vocab, bits;
@@ -37,90 +44,184 @@ struct SampleArgs {
     float* logprobs;
 };
 
-// A logit's bits in an order that is the values': -inf least, NaN as -inf, -0
-// as 0.
+// A logit as the sampler sees it: NaN is -inf, -0 is 0.
+__device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : -INFINITY; }
+// Its bits in an order that is the values'; -inf has the least.
 __device__ __forceinline__ uint32_t order_key(float x) {
-    x = x == x ? x + 0.0f : -INFINITY;
     const uint32_t b = __float_as_uint(x);
     return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu));
 }
-constexpr uint32_t kLeastKey = 0x007fffffu;  // -inf's
 
-// 2^z for z <= 0 in 64 bits: 2^f, |f| <= 1/2, by its Taylor series (the first
-// term left out is below 2^-56), scaled by the whole part.
-__device__ __forceinline__ double exp2_64(double z) {
-    if (!(z > -1000.0)) return 0.0;
-    const double n = rint(z), x = (z - n) * 0.69314718055994530942;
-    double p = 1.0 / 6227020800.0;
-    p = fma(p, x, 1.0 / 479001600.0);
-    p = fma(p, x, 1.0 / 39916800.0);
-    p = fma(p, x, 1.0 / 3628800.0);
-    p = fma(p, x, 1.0 / 362880.0);
-    p = fma(p, x, 1.0 / 40320.0);
-    p = fma(p, x, 1.0 / 5040.0);
-    p = fma(p, x, 1.0 / 720.0);
-    p = fma(p, x, 1.0 / 120.0);
-    p = fma(p, x, 1.0 / 24.0);
-    p = fma(p, x, 1.0 / 6.0);
-    p = fma(p, x, 0.5);
-    p = fma(p, x, 1.0);
-    p = fma(p, x, 1.0);
-    return ldexp(p, static_cast<int>(n));
-}
+// 2^(i / 16).
+__device__ constexpr double kRoots[16] = {
+    1.0,                1.0442737824274138, 1.0905077326652577, 1.1387886347566916,
+    1.1892071150027210, 1.2418578120734840, 1.2968395546510096, 1.3542555469368927,
+    1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543,
+    1.6817928305074290, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
 
-// A row's weights: of value v (its key not the least), relative to the row's
-// maximum, T's reciprocal times log2 e in c.
+// A row's weights relative to its maximum: w = 2^(z / 16), z = (x - top) *
+// 16 log2 e / T: a root from the table, the rest by its Taylor series (the
+// first term left out is below 2^-51).
 struct Weigh {
     float top;
-    double c;
+    double c;  // 16 log2 e / T
     int bits;
-    __device__ double exact(float v) const {
-        if (v == top) return 1.0;  // +inf too
-        return exp2_64((static_cast<double>(v) - static_cast<double>(top)) * c);
+    const double* roots;  // kRoots in LDS
+    __device__ __forceinline__ double operator()(float x) const {
+        const double d = x == top ? 0.0 : static_cast<double>(x) - static_cast<double>(top);
+        const double z = fmax(d * c, -65536.0);  // 2^-4096 is 0
+        const double n = rint(z);
+        const double y = (z - n) * (0.69314718055994530942 / 16);
+        double p = fma(y, 1.0 / 720.0, 1.0 / 120.0);
+        p = fma(p, y, 1.0 / 24.0);
+        p = fma(p, y, 1.0 / 6.0);
+        p = fma(p, y, 0.5);
+        p = fma(p, y, 1.0);
+        p = fma(p, y, 1.0);
+        const int i = static_cast<int>(n);
+        return ldexp(p * roots[i & 15], i >> 4);
     }
-    __device__ u64 whole(double w) const { return static_cast<u64>(rint(ldexp(w, bits))); }
-    __device__ u64 operator()(uint32_t key) const {
-        return key <= kLeastKey ? 0 : whole(exact(key_value(key)));
+    __device__ __forceinline__ u64 whole(float x) const {
+        return static_cast<u64>(rint(ldexp((*this)(x), bits)));
     }
 };
 
-__device__ __forceinline__ u64 shfl_up64(u64 v, int d) {
-    const uint32_t lo = __shfl_up(static_cast<uint32_t>(v), d, kWave);
-    const uint32_t hi = __shfl_up(static_cast<uint32_t>(v >> 32), d, kWave);
-    return static_cast<u64>(hi) << 32 | lo;
-}
-__device__ __forceinline__ u64 wave_scan64(u64 v) {  // inclusive
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {  // inclusive
     const int lane = threadIdx.x % kWave;
+#pragma unroll
     for (int d = 1; d < kWave; d *= 2) {
-        const u64 o = shfl_up64(v, d);
+        const T o = __shfl_up(v, d, kWave);
         if (lane >= d) v += o;
     }
     return v;
 }
 
-// One workgroup a row.
-__global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a) {
-    __shared__ u64 hist[256];
-    __shared__ u64 seg_sum[kMaxSegments];
-    __shared__ uint32_t seg_tie[kMaxSegments];
-    __shared__ uint32_t s_key;
-    __shared__ u64 s_left, s_total, s_target;
-    __shared__ uint32_t s_ties;
-    __shared__ int s_seg;
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid % kWave, V = a.vocab;
-    const float* x = a.logits + r * a.stride;
+struct SampleShared {
+    u64 weight[kBins];
+    uint32_t count[kBins];
+    u64 list_w[kList];
+    uint32_t list[kList];
+    double roots[16];
+    double part[kSampleWaves];
+    u64 part64[kSampleWaves];
+    float part_hi[kSampleWaves], part_lo[kSampleWaves];
+    uint32_t part_n[kSampleWaves];
+    uint32_t n, key, ties;
+    u64 left;
+    int token, last;
+};
 
-    if (tid == 0) s_key = 0;
+// Chunks a wave whose row LDS (160 KB) holds beside SampleShared.
+constexpr int kHeldChunks = 8;
+static_assert(sizeof(SampleShared) + kHeldChunks * kSampleWaves * kChunk * sizeof(float) <= 160 * 1024);
+
+template <class T>
+__device__ __forceinline__ T shfl(T v, int lane) { return __shfl(v, lane, kWave); }
+
+// Exclusive prefix of v over the workgroup's threads, and the total.
+template <class T>
+__device__ __forceinline__ T block_prefix(T v, T* part, T& total) {
+    const T in = wave_scan(v);
+    const int wave = threadIdx.x / kWave;
     __syncthreads();
-    uint32_t mine = 0;
-    for (int i = tid; i < V; i += kSampleThreads) mine = max(mine, order_key(x[i]));
-    atomicMax(&s_key, mine);
+    if (threadIdx.x % kWave == kWave - 1) part[wave] = in;
     __syncthreads();
-    const uint32_t top = s_key;
-    if (top <= kLeastKey) {
+    T before = 0;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < kSampleWaves; ++i) {
+        const T p = part[i];
+        before += i < wave ? p : T(0);
+        total += p;
+    }
+    return before + in - v;
+}
+
+// A row's logits, cleaned. HELD: kept in LDS, read from memory once.
+template <bool HELD>
+struct Row {
+    const float* x;
+    float* held;
+    int vocab, pre, chunks;  // pre: floats from 16 bytes' alignment to the row
+
+    __device__ __forceinline__ int position(int c) const {
+        return ((threadIdx.x / kWave) * chunks + c) * kChunk + 4 * (threadIdx.x % kWave);
+    }
+    __device__ __forceinline__ float load(int pos) const {
+        const int i = pos - pre;
+        return i >= 0 && i < vocab ? clean(x[i]) : -INFINITY;
+    }
+    __device__ __forceinline__ float4 load4(int pos) const {
+        if (pos >= pre && pos + 4 <= pre + vocab) {
+            const float4 v = *reinterpret_cast<const float4*>(x + (pos - pre));
+            return make_float4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
+        }
+        return make_float4(load(pos), load(pos + 1), load(pos + 2), load(pos + 3));
+    }
+    __device__ __forceinline__ float at(int pos) const {
+        if constexpr (HELD) return held[pos];
+        return load(pos);
+    }
+    // f(x) of every logit of this thread; KEEP: the pass that fills `held`.
+    template <bool KEEP = false, class Fn>
+    __device__ __forceinline__ void each(Fn f) const {
+        constexpr int U = 4;  // vectors in flight
+        for (int c = 0; c < chunks; c += U) {
+            float4 v[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const int pos = position(min(c + i, chunks - 1));
+                if constexpr (HELD && !KEEP)
+                    v[i] = *reinterpret_cast<const float4*>(held + pos);
+                else
+                    v[i] = load4(pos);
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (c + i >= chunks) break;
+                if constexpr (HELD && KEEP)
+                    *reinterpret_cast<float4*>(held + position(c + i)) = v[i];
+                f(v[i].x);
+                f(v[i].y);
+                f(v[i].z);
+                f(v[i].w);
+            }
+        }
+    }
+};
+
+template <bool HELD>
+__global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a) {
+    __shared__ SampleShared s;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    extern __shared__ __attribute__((aligned(16))) float held[];
+    Row<HELD> row;
+    row.held = held;
+    row.x = a.logits + r * a.stride;
+    row.vocab = a.vocab;
+    row.pre = static_cast<int>(reinterpret_cast<uintptr_t>(row.x) / 4 % 4);
+    row.chunks = (a.vocab + row.pre + kSampleWaves * kChunk - 1) / (kSampleWaves * kChunk);
+    if (tid < 16) s.roots[tid] = kRoots[tid];
+
+    // The maximum, and the least of the threads' maxima.
+    float most = -INFINITY;
+    row.template each<true>([&](float x) { most = fmaxf(most, x); });
+    float top = wave_max(most), low = -wave_max(-most);
+    if (lane == 0) {
+        s.part_hi[wave] = top;
+        s.part_lo[wave] = low;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSampleWaves; ++i) {
+        top = fmaxf(top, s.part_hi[i]);
+        low = fminf(low, s.part_lo[i]);
+    }
+    if (top == -INFINITY) {
         if (tid == 0) {
             a.tokens[r] = -1;
             if (a.logprobs) a.logprobs[r] = -INFINITY;
@@ -129,179 +230,303 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
     }
     const float T = a.temperature ? a.temperature[r] : 1.0f;
     const bool greedy = !(T > 0.0f);
-    const Weigh weigh{key_value(top), greedy ? 0.0 : 1.4426950408889634074 / T, a.bits};
+    const Weigh weigh{top, greedy ? 0.0 : 16 * 1.4426950408889634074 / T, a.bits, s.roots};
 
-    // The last token kept: value thr, `ties` of that value.
-    uint32_t thr = kLeastKey + 1, ties = V;
+    // The last token kept: value thr, the first `ties` of that value.
+    float thr = -INFINITY;
+    uint32_t ties = 0;
+
     // Radix selection from the top: the value at which the running sum of
-    // `amount` over falling values reaches `target`, and what is left of the
+    // amount(x) over falling values reaches `target`, and what is left of the
     // target for the tokens of just that value.
-    auto select = [&](u64 target, auto amount) {
+    auto radix = [&](u64 target, auto amount) {
         uint32_t prefix = 0;
         u64 left = target;
         for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
             __syncthreads();
-            for (int i = tid; i < V; i += kSampleThreads) {
-                const uint32_t k = order_key(x[i]);
-                if (k > kLeastKey && (shift == 24 || k >> (shift + 8) == prefix))
-                    atomicAdd(&hist[k >> shift & 255], amount(k));
-            }
+            if (tid < 256) s.weight[tid] = 0;
+            __syncthreads();
+            row.each([&](float x) {
+                const uint32_t k = order_key(x);
+                if (x > -INFINITY && (shift == 24 || k >> (shift + 8) == prefix))
+                    atomicAdd(&s.weight[k >> shift & 255], amount(x));
+            });
             __syncthreads();
             if (tid == 0) {
                 u64 l = left;
                 int b = 255;
-                while (b > 0 && hist[b] < l) l -= hist[b--];
-                s_left = l;
-                s_key = prefix << 8 | b;
+                while (b > 0 && s.weight[b] < l) l -= s.weight[b--];
+                s.left = l;
+                s.key = prefix << 8 | b;
             }
             __syncthreads();
-            prefix = s_key;
-            left = s_left;
-            __syncthreads();
+            prefix = s.key;
+            left = s.left;
         }
-        thr = prefix;
+        thr = key_value(prefix);
         return left;
     };
+    // The histogram's bin of x; inv: bins over the range they cover.
+    auto bin_of = [&](float x, float inv) {
+        const float b = x == top ? 0.0f : (top - x) * inv;
+        return b < kBins - 1 ? static_cast<int>(b) : kBins - 1;
+    };
+    // The bin in which the running sum reaches `target` and what is left of
+    // it there; two bins a thread.
+    auto border = [&](const auto& bins, auto* part, u64 target, u64& left) {
+        const auto b0 = bins[2 * tid], b1 = bins[2 * tid + 1];
+        auto total = b0;
+        const u64 before = block_prefix(b0 + b1, part, total);
+        if (before < target && before + b0 + b1 >= target) {
+            const bool second = before + b0 < target;
+            s.n = 2 * tid + second;
+            s.left = target - before - (second ? b0 : 0);
+        }
+        __syncthreads();
+        const int bin = s.n;
+        left = s.left;
+        __syncthreads();
+        if (tid == 0) s.n = 0;
+        __syncthreads();
+        return bin;
+    };
+
     const int k = a.top_k ? a.top_k[r] : 0;
     if (greedy) {
         thr = top;
         ties = 1;
-    } else if (k > 0 && k < V) {
-        // Fewer than k tokens that can be drawn: the filter is off.
-        if (tid == 0) s_total = 0;
+    } else if (k > 0 && k < a.vocab) {
+        // Where every thread has a maximum, k of them are at least the least
+        // one, so only tokens from there on need be counted.
+        float floor = low;
+        if (low == -INFINITY || k > kSampleThreads) {
+            float least = INFINITY;
+            row.each([&](float x) { least = x > -INFINITY ? fminf(least, x) : least; });
+            least = -wave_max(-least);
+            __syncthreads();
+            if (lane == 0) s.part_lo[wave] = least;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kSampleWaves; ++i) least = fminf(least, s.part_lo[i]);
+            floor = least;
+        }
+        const float inv = fminf((kBins - 1) / (top - floor), 3e38f);
+        for (int i = tid; i < kBins; i += kSampleThreads) s.count[i] = 0;
         __syncthreads();
-        u64 n = 0;
-        for (int i = tid; i < V; i += kSampleThreads) n += order_key(x[i]) > kLeastKey;
-        atomicAdd(&s_total, n);
+        row.each([&](float x) {
+            if (x >= floor) atomicAdd(&s.count[bin_of(x, inv)], 1u);
+        });
         __syncthreads();
-        const u64 all = s_total;
-        __syncthreads();
-        if (all > static_cast<u64>(k)) ties = select(k, [](uint32_t) { return u64{1}; });
+        u64 left = 0;
+        uint32_t all = 0;
+        // Fewer tokens than k that can be drawn: the filter is off.
+        (void)block_prefix(s.count[2 * tid] + s.count[2 * tid + 1], s.part_n, all);
+        if (all >= static_cast<uint32_t>(k)) {
+            const int bin = border(s.count, s.part_n, k, left);
+            row.each([&](float x) {
+                if (x >= floor && bin_of(x, inv) == bin) {
+                    const uint32_t i = atomicAdd(&s.n, 1u);
+                    if (i < kList) s.list[i] = order_key(x);
+                }
+            });
+            __syncthreads();
+            const uint32_t n = s.n;
+            if (n <= kList) {
+                if (static_cast<uint32_t>(tid) < n) {
+                    const uint32_t mine = s.list[tid];
+                    uint32_t above = 0, equal = 0;
+                    for (uint32_t i = 0; i < n; ++i) {
+                        above += s.list[i] > mine;
+                        equal += s.list[i] == mine;
+                    }
+                    if (above < left && above + equal >= left) {
+                        s.key = mine;
+                        s.ties = static_cast<uint32_t>(left) - above;
+                    }
+                }
+                __syncthreads();
+                thr = key_value(s.key);
+                ties = s.ties;
+            } else {
+                ties = static_cast<uint32_t>(radix(k, [](float) { return u64{1}; }));
+            }
+        }
     }
+
     const float top_p = a.top_p ? a.top_p[r] : 1.0f;
     if (!greedy && top_p < 1.0f) {
-        if (tid == 0) s_total = 0;
+        // Bins of 1/64 of a factor of two in weight, the last one from 2^-32.
+        const float inv = static_cast<float>(fmin(weigh.c * (64.0 / 16.0), 3e38));
         __syncthreads();
-        u64 n = 0;
-        for (int i = tid; i < V; i += kSampleThreads) {
-            const uint32_t key = order_key(x[i]);
-            if (key > thr) n += weigh(key);
-        }
-        atomicAdd(&s_total, n);
-        // Every token of the threshold's value, up to the ties kept.
-        if (tid == 0) s_ties = 0;
+        for (int i = tid; i < kBins; i += kSampleThreads) s.weight[i] = 0;
         __syncthreads();
-        uint32_t c = 0;
-        for (int i = tid; i < V; i += kSampleThreads) c += order_key(x[i]) == thr;
-        atomicAdd(&s_ties, c);
+        row.each([&](float x) {
+            if (x > thr) {
+                const u64 w = weigh.whole(x);
+                if (w) atomicAdd(&s.weight[bin_of(x, inv)], w);
+            }
+        });
+        if (tid == 0 && ties) atomicAdd(&s.weight[bin_of(thr, inv)], ties * weigh.whole(thr));
         __syncthreads();
-        const u64 total = s_total + min(ties, s_ties) * weigh(thr);
-        __syncthreads();
-        u64 target = static_cast<u64>(ceil(static_cast<double>(fmaxf(top_p, 0.0f)) *
-                                           static_cast<double>(total)));
+        u64 total = 0, left = 0;
+        (void)block_prefix(s.weight[2 * tid] + s.weight[2 * tid + 1], s.part64, total);
+        u64 target = static_cast<u64>(
+            ceil(static_cast<double>(fmaxf(top_p, 0.0f)) * static_cast<double>(total)));
         target = max(u64{1}, min(target, total));
-        const u64 left = select(target, weigh);
-        const u64 w = max(u64{1}, weigh(thr));
-        ties = static_cast<uint32_t>((left + w - 1) / w);
+        const int bin = border(s.weight, s.part64, target, left);
+        row.each([&](float x) {
+            if (x >= thr && x > -INFINITY && bin_of(x, inv) == bin) {
+                const u64 w = weigh.whole(x);
+                if (w) {
+                    const uint32_t i = atomicAdd(&s.n, 1u);
+                    if (i < kList) {
+                        s.list[i] = order_key(x);
+                        s.list_w[i] = w;
+                    }
+                }
+            }
+        });
+        __syncthreads();
+        const uint32_t n = s.n;
+        if (n <= kList) {
+            if (static_cast<uint32_t>(tid) < n) {
+                const uint32_t mine = s.list[tid];
+                const u64 w = s.list_w[tid];
+                u64 above = 0;
+                uint32_t equal = 0;
+                for (uint32_t i = 0; i < n; ++i) {
+                    above += s.list[i] > mine ? s.list_w[i] : 0;
+                    equal += s.list[i] == mine;
+                }
+                if (ties && key_value(mine) == thr) equal = min(equal, ties);
+                if (above < left && above + equal * w >= left) {
+                    s.key = mine;
+                    s.ties = static_cast<uint32_t>((left - above + w - 1) / w);
+                }
+            }
+            __syncthreads();
+            thr = key_value(s.key);
+            ties = s.ties;
+        } else {
+            const u64 rest = radix(target, [&](float x) { return weigh.whole(x); });
+            const u64 w = max(u64{1}, weigh.whole(thr));
+            ties = static_cast<uint32_t>((rest + w - 1) / w);
+        }
     }
     const float mp = a.min_p ? a.min_p[r] : 0.0f;
     const double min_p = mp > 0.0f ? fmin(static_cast<double>(mp), 1.0) : 0.0;
-    auto kept = [&](uint32_t key) -> u64 {  // the weight of a token above the threshold
-        if (key <= kLeastKey || key < thr) return 0;
-        const double w = weigh.exact(key_value(key));
-        return w >= min_p ? weigh.whole(w) : 0;
+    auto kept = [&](float x) {  // the weight of a token that top-k and top-p keep
+        const double w = weigh(x);
+        return w >= min_p ? w : 0.0;
     };
+    const double wt = thr > -INFINITY ? kept(thr) : 0.0;
 
-    // Each segment's kept weight above the threshold and tokens at it.
-    const int segs = (V + kSegment - 1) / kSegment;
-    for (int s = tid / kWave; s < segs; s += kSampleWaves) {
-        u64 sum = 0;
-        uint32_t tie = 0;
-        for (int i = 0; i < 4; ++i) {
-            const int at = s * kSegment + 4 * lane + i;
-            if (at >= V) continue;
-            const uint32_t key = order_key(x[at]);
-            if (key > thr) sum += kept(key);
-            tie += key == thr;
-        }
-        sum = wave_scan64(sum);
-        for (int d = 1; d < kWave; d *= 2) {
-            const uint32_t o = __shfl_up(tie, d, kWave);
-            if (lane >= d) tie += o;
-        }
-        if (lane == kWave - 1) {
-            seg_sum[s] = sum;
-            seg_tie[s] = tie;
-        }
-    }
+    // Each wave's kept weight above the threshold and its tokens at it.
+    double sum = 0.0;
+    uint32_t at_thr = 0;
+    row.each([&](float x) {
+        if (x > thr) sum += kept(x);
+        at_thr += x == thr && ties;
+    });
+    sum = shfl(wave_scan(sum), kWave - 1);
+    at_thr = shfl(wave_scan(at_thr), kWave - 1);
     __syncthreads();
-    const u64 wt = kept(thr);
-    if (tid == 0) {
-        u64 total = 0;
+    if (lane == 0) {
+        s.part[wave] = sum;
+        s.part_n[wave] = at_thr;
+    }
+    if (tid == 0) s.token = s.last = -1;
+    __syncthreads();
+    double total = 0.0;
+    {
         uint32_t left = ties;
-        for (int s = 0; s < segs; ++s) {
-            const uint32_t n = min(left, seg_tie[s]);
+#pragma unroll
+        for (int i = 0; i < kSampleWaves; ++i) {
+            const uint32_t n = min(left, s.part_n[i]);
             left -= n;
-            total += seg_sum[s] + n * wt;
+            total += s.part[i] + n * wt;
         }
-        const float u = a.u[r];
-        u64 target = u > 0.0f ? static_cast<u64>(static_cast<double>(u) * static_cast<double>(total)) : 0;
-        target = min(target, total - 1);
-        u64 sum = 0;
-        left = ties;
-        int s = 0;
-        for (; s < segs - 1; ++s) {
-            const uint32_t n = min(left, seg_tie[s]);
-            const u64 w = seg_sum[s] + n * wt;
-            if (sum + w > target) break;
-            left -= n;
-            sum += w;
-        }
-        s_seg = s;
-        s_target = target - sum;
-        s_ties = left;
-        s_total = total;
     }
-    __syncthreads();
-    if (tid >= kWave) return;
-    // The segment's values in order: one wave, four a lane.
-    uint32_t key[4], tie[4], before = 0;
-    for (int i = 0; i < 4; ++i) {
-        const int at = s_seg * kSegment + 4 * lane + i;
-        key[i] = at < V ? order_key(x[at]) : 0;
-        tie[i] = key[i] == thr;
-        before += tie[i];
-    }
-    uint32_t run = before;
-    for (int d = 1; d < kWave; d *= 2) {
-        const uint32_t o = __shfl_up(run, d, kWave);
-        if (lane >= d) run += o;
-    }
-    run -= before;
-    u64 w[4], sum = 0;
-    for (int i = 0; i < 4; ++i) {
-        w[i] = key[i] > thr ? kept(key[i]) : tie[i] && run < s_ties ? wt : 0;
-        run += tie[i];
-        sum += w[i];
-    }
-    u64 c = wave_scan64(sum) - sum;
-    for (int i = 0; i < 4; ++i) {
-        if (w[i] && c <= s_target && c + w[i] > s_target) {
-            a.tokens[r] = s_seg * kSegment + 4 * lane + i;
-            if (a.logprobs) {
-                const double p = ldexp(weigh.exact(key_value(key[i])), a.bits);
-                a.logprobs[r] = static_cast<float>(log(p / static_cast<double>(s_total)));
+    const float u = a.u[r];
+    double target = u > 0.0f ? fmin(static_cast<double>(u), 1.0) * total : 0.0;
+    int pick = 0;
+    uint32_t left = ties;
+    {
+        // The first wave whose running sum passes the target (the last with
+        // any weight where rounding leaves none).
+        double run = 0.0, pick_run = 0.0;
+        uint32_t l = ties;
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < kSampleWaves; ++i) {
+            const uint32_t n = min(l, s.part_n[i]);
+            const double w = s.part[i] + n * wt;
+            if (!found && w > 0.0) {
+                pick = i;
+                pick_run = run;
+                left = l;
+                found = run + w > target;
             }
+            l -= n;
+            run += w;
         }
-        c += w[i];
+        target -= pick_run;
     }
+    // That wave's run of the row, `each` consecutive logits a thread.
+    const int span = row.chunks * kChunk, each = (span + kSampleThreads - 1) / kSampleThreads;
+    const int from = pick * span + tid * each, to = min(from + each, (pick + 1) * span);
+    double mine = 0.0;
+    uint32_t n = 0;
+    for (int p = from; p < to; ++p) {
+        const float x = row.at(p);
+        if (x > thr) mine += kept(x);
+        n += x == thr && ties;
+    }
+    uint32_t dummy_n = 0;
+    const uint32_t n_before = block_prefix(n, s.part_n, dummy_n);
+    uint32_t here = left > n_before ? min(left - n_before, n) : 0;
+    mine += here * wt;
+    double dummy = 0.0;
+    const double before = block_prefix(mine, s.part, dummy);
+    const bool hit = mine > 0.0 && before <= target && before + mine > target;
+    if (hit) s.token = 1;
+    if (mine > 0.0) atomicMax(&s.last, tid);
+    __syncthreads();
+    // The scan's rounding may leave a gap that the target falls into: the
+    // last thread with any weight then takes it.
+    if (!(hit || (s.token < 0 && tid == s.last))) return;
+    double run = before;
+    int token = -1;
+    double w_token = 0.0;
+    for (int p = from; p < to; ++p) {
+        const float x = row.at(p);
+        double w = 0.0;
+        if (x > thr) {
+            w = kept(x);
+        } else if (x == thr && here > 0) {
+            --here;
+            w = wt;
+        }
+        if (!(w > 0.0)) continue;
+        token = p - row.pre;
+        w_token = w;
+        run += w;
+        if (run > target) break;
+    }
+    a.tokens[r] = token;
+    if (a.logprobs) a.logprobs[r] = static_cast<float>(log(w_token / total));
 }
 
 std::size_t sample_scratch(std::size_t, std::size_t) { return 0; }
 
 void run_sample(const SampleArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL(sample_row_kernel, dim3(a.rows), dim3(kSampleThreads), 0, stream, a);
+    // Rows that fit LDS beside the rest, up to three floats off their 16 bytes.
+    const int per = kSampleWaves * kChunk, chunks = (a.vocab + 3 + per - 1) / per;
+    if (chunks <= kHeldChunks)
+        hipLaunchKernelGGL(sample_row_kernel<true>, dim3(a.rows), dim3(kSampleThreads),
+                           chunks * per * sizeof(float), stream, a);
+    else
+        hipLaunchKernelGGL(sample_row_kernel<false>, dim3(a.rows), dim3(kSampleThreads), 0, stream, a);
 }
 
 }  // namespace
