@@ -472,59 +472,78 @@ def paged_check(shape: PagedShape) -> None:
 
 
 def _here(stream):
-    """The call's stream, a context that allocates on it, and the current device."""
+    """The current device and the address of the call's stream on it."""
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
+    if stream is None:
+        device = torch.cuda.current_device()
+        return device, torch._C._cuda_getCurrentRawStream(device)
     device = torch.cuda.current_device()
-    if s.device.index != device:
-        raise InvalidArgument(EM_EINVAL, f"the stream is on {s.device}, the current device is "
-                                         f"cuda:{device}")
-    return s, torch.cuda.stream(s), device
+    if stream.device.index != device:
+        raise InvalidArgument(EM_EINVAL, f"the stream is on {stream.device}, the current device "
+                                         f"is cuda:{device}")
+    return device, int(stream.cuda_stream)
 
 
-def _on(t, what, dtype, device, shape=None):
+def _new(make, stream, *size, dtype):
+    """A tensor for the call's own use or its result, allocated on its stream
+    so that the allocator does not hand it on before the call has run."""
+    import torch
+    if stream is None:
+        return make(size, dtype=dtype, device="cuda")
+    with torch.cuda.stream(stream):
+        return make(size, dtype=dtype, device="cuda")
+
+
+def _on(t, what, dtype, device, *shape):
     """t's address: of type `dtype`, on the current device, contiguous and of `shape`."""
-    if not t.is_cuda or t.device.index != device or t.dtype != dtype or not t.is_contiguous() or \
-            (shape is not None and tuple(t.shape) != tuple(shape)):
-        of = "" if shape is None else " of shape " + "x".join(map(str, shape))
-        raise InvalidArgument(EM_EINVAL, f"{what}: expected a contiguous {dtype} tensor{of} on "
+    if t.dtype is not dtype or t.get_device() != device or t.shape != shape or \
+            not t.is_contiguous():
+        raise InvalidArgument(EM_EINVAL, f"{what}: expected a contiguous {dtype} tensor of shape "
+                                         f"{'x'.join(map(str, shape))} on cuda:{device}")
+    return t.data_ptr()
+
+
+def _scratch_of(t, dtype, need, device):
+    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous() or \
+            t.numel() < need:
+        raise InvalidArgument(EM_EINVAL, f"scratch: expected {need} contiguous {dtype} on "
                                          f"cuda:{device}")
     return t.data_ptr()
 
 
-def _rows_of(t, what, rows, width, device):
-    """(address, floats between rows) of a 2-D fp32 tensor of `rows` rows at
+def _rows_of(t, what, dtype, rows, width, device):
+    """(address, elements between rows) of a 2-D tensor of `rows` rows at
     least `width` wide, its columns together, e.g. a slice of the qkv product's."""
-    import torch
-    if not t.is_cuda or t.device.index != device or t.dtype != torch.float32 or t.dim() != 2 or \
-            t.shape[0] != rows or t.shape[1] < width or (width > 1 and t.stride(1) != 1):
-        raise InvalidArgument(EM_EINVAL, f"{what}: expected {rows} fp32 rows of {width} on "
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not dtype or t.get_device() != device or len(shape) != 2 or \
+            shape[0] != rows or shape[1] < width or (width > 1 and stride[1] != 1):
+        raise InvalidArgument(EM_EINVAL, f"{what}: expected {rows} {dtype} rows of {width} on "
                                          f"cuda:{device}")
-    return t.data_ptr(), (t.stride(0) if rows > 1 else max(t.stride(0), width))
+    return t.data_ptr(), (stride[0] if rows > 1 else max(stride[0], width))
+
+
+_CACHE_DTYPES: list = []
 
 
 def _paged_args(shape, row_start, lengths, page_table, key_cache, value_cache, device):
     import torch
-    _check(lib().em_paged_check(ctypes.byref(shape)))
-    n = lengths.shape[0]
-    if page_table.dim() != 2 or page_table.shape[0] != n or \
-            page_table.shape[1] < shape.max_pages or not page_table.is_cuda or \
-            page_table.device.index != device or page_table.dtype != torch.int32 or \
-            (shape.max_pages > 1 and page_table.stride(1) != 1):
-        raise InvalidArgument(EM_EINVAL, f"page_table: expected {n} int32 rows of "
-                                         f"{shape.max_pages} on cuda:{device}")
-    stride = page_table.stride(0) if n > 1 else max(page_table.stride(0), shape.max_pages)
-    batch = PagedBatch(n, _on(row_start, "row_start", torch.int32, device, (n + 1,)),
-                       _on(lengths, "lengths", torch.int32, device, (n,)), page_table.data_ptr(),
-                       stride)
-    dtype = {0: torch.float32, 1: torch.float16, 2: torch.bfloat16}[shape.type]
+    if not _CACHE_DTYPES:
+        _CACHE_DTYPES.extend((torch.float32, torch.float16, torch.bfloat16))
+    int32, n, kind = torch.int32, lengths.shape[0], shape.type
+    if not 0 <= kind < 3:
+        _check(lib().em_paged_check(ctypes.byref(shape)))
+    table, stride = _rows_of(page_table, "page_table", int32, n, shape.max_pages, device)
+    batch = PagedBatch(n, _on(row_start, "row_start", int32, device, n + 1),
+                       _on(lengths, "lengths", int32, device, n), table, stride)
     # One past the last element the shape reaches.
     last = (shape.n_pages - 1) * shape.page_stride + (shape.page_size - 1) * shape.slot_stride + \
         (shape.n_kv_heads - 1) * shape.head_stride + shape.head_size
+    dtype = _CACHE_DTYPES[kind]
     for t, what in ((key_cache, "key_cache"), (value_cache, "value_cache")):
-        if not t.is_cuda or t.device.index != device or t.dtype != dtype:
+        if t.dtype is not dtype or t.get_device() != device:
             raise InvalidArgument(EM_EINVAL, f"{what}: expected {dtype} on cuda:{device}")
-        if 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride())) < last:
+        if not (t.is_contiguous() and t.numel() >= last) and \
+                1 + sum((m - 1) * st for m, st in zip(t.shape, t.stride())) < last:
             raise InvalidArgument(EM_EINVAL, f"{what}: the shape reaches {last} elements, past "
                                              "the tensor's last")
     return batch
@@ -537,30 +556,30 @@ def paged_append(shape: PagedShape, row_start, lengths, page_table, q, k, v, key
     rotation). Returns the rotated queries: q_out (q itself to rotate in
     place) or a new tensor."""
     import torch
-    s, ctx, device = _here(stream)
+    f32 = torch.float32
+    device, s = _here(stream)
     batch = _paged_args(shape, row_start, lengths, page_table, key_cache, value_cache, device)
-    rows, dim, kv = k.shape[0], shape.n_heads * shape.head_size, shape.n_kv_heads * shape.head_size
+    size = shape.head_size
+    rows, dim, kv = k.shape[0], shape.n_heads * size, shape.n_kv_heads * size
     qp, qs, op, os_ = None, 0, None, 0
     if q is not None:
-        qp, qs = _rows_of(q, "q", rows, dim, device)
+        qp, qs = _rows_of(q, "q", f32, rows, dim, device)
         if q_out is None:
-            with ctx:
-                q_out = torch.empty((rows, dim), dtype=torch.float32, device=q.device)
-        op, os_ = _rows_of(q_out, "q_out", rows, dim, device)
-    kp, ks = _rows_of(k, "k", rows, kv, device)
-    vp, vs = _rows_of(v, "v", rows, kv, device)
+            q_out = _new(torch.empty, stream, rows, dim, dtype=f32)
+        op, os_ = _rows_of(q_out, "q_out", f32, rows, dim, device)
+    kp, ks = _rows_of(k, "k", f32, rows, kv, device)
+    vp, vs = _rows_of(v, "v", f32, rows, kv, device)
     fp, rotary = None, 0
     if freq is not None and freq.numel():
-        fp, rotary = _on(freq, "freq", torch.float32, device, (freq.numel(),)), 2 * freq.numel()
-    _check(lib().em_paged_append(ctypes.byref(shape), ctypes.byref(batch), rows, qp, qs, kp, ks,
-                                 vp, vs, fp, rotary, int(bool(halves)), op, os_,
-                                 key_cache.data_ptr(), value_cache.data_ptr(),
-                                 int(s.cuda_stream) or None))
+        fp, rotary = _on(freq, "freq", f32, device, freq.numel()), 2 * freq.numel()
+    _check(lib().em_paged_append(shape, batch, rows, qp, qs, kp, ks, vp, vs, fp, rotary,
+                                 1 if halves else 0, op, os_, key_cache.data_ptr(),
+                                 value_cache.data_ptr(), s))
     return q_out
 
 
 def paged_attention_scratch_floats(shape: PagedShape, n_seqs: int, rows: int) -> int:
-    return int(lib().em_paged_attention_scratch_floats(ctypes.byref(shape), n_seqs, rows))
+    return int(lib().em_paged_attention_scratch_floats(shape, n_seqs, rows))
 
 
 def paged_attention(shape: PagedShape, row_start, lengths, page_table, q, key_cache, value_cache,
@@ -568,23 +587,20 @@ def paged_attention(shape: PagedShape, row_start, lengths, page_table, q, key_ca
     """em_paged_attention on torch tensors: q is 2-D fp32, a row-strided view
     allowed. A new `out` holds zeros in rows that are no sequence's."""
     import torch
-    s, ctx, device = _here(stream)
+    f32 = torch.float32
+    device, s = _here(stream)
     batch = _paged_args(shape, row_start, lengths, page_table, key_cache, value_cache, device)
     rows, dim = q.shape[0], shape.n_heads * shape.head_size
-    qp, qs = _rows_of(q, "q", rows, dim, device)
+    qp, qs = _rows_of(q, "q", f32, rows, dim, device)
     need = paged_attention_scratch_floats(shape, batch.n_seqs, rows)
-    with ctx:
-        if out is None:
-            out = torch.zeros((rows, dim), dtype=torch.float32, device=q.device)
-        if scratch is None:
-            scratch = torch.empty((max(1, need),), dtype=torch.float32, device=q.device)
-    op, os_ = _rows_of(out, "out", rows, dim, device)
-    sp = _on(scratch, "scratch", torch.float32, device)
-    if scratch.numel() < need:
-        raise InvalidArgument(EM_EINVAL, f"scratch: {scratch.numel()} floats, {need} needed")
-    _check(lib().em_paged_attention(ctypes.byref(shape), ctypes.byref(batch), rows, qp, qs,
-                                    key_cache.data_ptr(), value_cache.data_ptr(), op, os_,
-                                    scale, window, sp, int(s.cuda_stream) or None))
+    if out is None:
+        out = _new(torch.zeros, stream, rows, dim, dtype=f32)
+    if scratch is None:
+        scratch = _new(torch.empty, stream, max(1, need), dtype=f32)
+    op, os_ = _rows_of(out, "out", f32, rows, dim, device)
+    _check(lib().em_paged_attention(shape, batch, rows, qp, qs, key_cache.data_ptr(),
+                                    value_cache.data_ptr(), op, os_, scale, window,
+                                    _scratch_of(scratch, f32, need, device), s))
     return out
 
 
@@ -600,30 +616,26 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     u and the settings one value a row, top_k int32, the others fp32; None is
     off (temperature: 1). Returns (tokens int32, logprobs fp32)."""
     import torch
-    s, ctx, device = _here(stream)
+    f32, i32 = torch.float32, torch.int32
+    device, s = _here(stream)
     if logits.dim() != 2:
         raise InvalidArgument(EM_EINVAL, "logits: expected 2-D fp32")
     rows, vocab = logits.shape
-    lp, ls = _rows_of(logits, "logits", rows, vocab, device)
-    opt = lambda t, what, dt: None if t is None else _on(t, what, dt, device, (rows,))
-    settings = Sampling(opt(temperature, "temperature", torch.float32),
-                        opt(top_k, "top_k", torch.int32), opt(top_p, "top_p", torch.float32),
-                        opt(min_p, "min_p", torch.float32))
+    lp, ls = _rows_of(logits, "logits", f32, rows, vocab, device)
+    opt = lambda t, what, dt: None if t is None else _on(t, what, dt, device, rows)
+    settings = Sampling(opt(temperature, "temperature", f32), opt(top_k, "top_k", i32),
+                        opt(top_p, "top_p", f32), opt(min_p, "min_p", f32))
     need = sample_scratch_bytes(rows, vocab)
-    with ctx:
-        if tokens is None:
-            tokens = torch.empty((rows,), dtype=torch.int32, device=logits.device)
-        if logprobs is None:
-            logprobs = torch.empty((rows,), dtype=torch.float32, device=logits.device)
-        if scratch is None:
-            scratch = torch.empty((max(1, need),), dtype=torch.uint8, device=logits.device)
-    sp = _on(scratch, "scratch", torch.uint8, device)
-    if scratch.numel() < need:
-        raise InvalidArgument(EM_EINVAL, f"scratch: {scratch.numel()} bytes, {need} needed")
-    _check(lib().em_sample(rows, vocab, lp, ls, _on(u, "u", torch.float32, device, (rows,)),
-                           ctypes.byref(settings), _on(tokens, "tokens", torch.int32, device, (rows,)),
-                           _on(logprobs, "logprobs", torch.float32, device, (rows,)), sp,
-                           int(s.cuda_stream) or None))
+    if tokens is None:
+        tokens = _new(torch.empty, stream, rows, dtype=i32)
+    if logprobs is None:
+        logprobs = _new(torch.empty, stream, rows, dtype=f32)
+    if scratch is None:
+        scratch = _new(torch.empty, stream, max(1, need), dtype=torch.uint8)
+    _check(lib().em_sample(rows, vocab, lp, ls, _on(u, "u", f32, device, rows), settings,
+                           _on(tokens, "tokens", i32, device, rows),
+                           _on(logprobs, "logprobs", f32, device, rows),
+                           _scratch_of(scratch, torch.uint8, need, device), s))
     return tokens, logprobs
 
 
