@@ -13,6 +13,7 @@
 // (Plan): the positions of all columns over the workgroups the card holds at
 // once give a run's length, a sequence's positions are cut into runs of about
 // that many, and blockIdx.x is looked up in the running number of items.
+#include <algorithm>
 #include <cmath>
 
 #include "paged.hpp"
@@ -272,7 +273,7 @@ __device__ __forceinline__ uint32_t slot_unit(const PagedArgs& p, int seq, int t
 // m, l: maximum (of log2 weights) and sum; o[i]: head dim lane + 64 i,
 // unnormalised.
 template <class T, int N>
-__device__ __noinline__ void plain_column(const PagedAttnArgs& a, int seq, int row, int head,
+__device__ __forceinline__ void plain_column(const PagedAttnArgs& a, int seq, int row, int head,
                                           int pq, int lo, int hi, int stride, float& m, float& l,
                                           float (&o)[N]) {
     const PagedArgs& p = a.p;
@@ -379,6 +380,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_few_kernel(
     constexpr int kRow = DP + 4;  // floats of a column in LDS
     __shared__ __attribute__((aligned(16))) float o_s[kWaves][kCols][kRow];
     __shared__ float2 ml_s[kWaves][kCols];
+    // fp32 keys and values take the registers that the query terms, the same
+    // in every wave, would need (148 spilled): those are read from LDS.
+    constexpr bool kQueryLds = KT == 3;
+    __shared__ __attribute__((aligned(16))) typename F::Frag q_s[kQueryLds ? C * NT * kWave : 1];
     const PagedArgs& p = a.p;
     const int tid = threadIdx.x, lane = tid % kWave, g = lane >> 4, j = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -408,7 +413,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_few_kernel(
     const int all_lo = a.window ? f.w.p0 + i1 + 1 - a.window : 0, all_hi = f.w.p0 + i0;
 
     // The column's query terms.
-    typename F::Frag q[C][NT];
+    typename F::Frag q[kQueryLds ? 1 : C][NT];
     uint32_t lost_q = 0, lost_v = 0;
     float top_q = 0.0f, unscale = 1.0f;
     {
@@ -440,7 +445,14 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_few_kernel(
                 for (int e = 0; e < 8; ++e) v[c][e] *= up;
         }
 #pragma unroll
-        for (int c = 0; c < C; ++c) split_terms(v[c], q[c], lost_q);
+        for (int c = 0; c < C; ++c) {
+            split_terms(v[c], q[kQueryLds ? 0 : c], lost_q);
+            if (kQueryLds && w == 0) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t) q_s[(c * NT + t) * kWave + lane] = q[0][t];
+            }
+        }
+        if (kQueryLds) __syncthreads();
     }
     // fp32 keys below 2^-109 drop bits worth up to 2^-134 each: nothing for a
     // query below 2^90. fp16's scale reaches down to 2^-106.
@@ -516,7 +528,16 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_few_kernel(
                 for (int c = 0; c < C; ++c) {
                     typename F::Frag kt[KT];
                     key_terms(k[y][c], kt);
-                    mma_terms(kt, q[c], s[y]);
+                    if constexpr (kQueryLds) {
+                        typename F::Frag qt[NT];
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) qt[t] = q_s[(c * NT + t) * kWave + lane];
+                        mma_terms(kt, qt, s[y]);
+                        // One split's terms at a time, not all of them in registers.
+                        __builtin_amdgcn_sched_barrier(0);
+                    } else {
+                        mma_terms(kt, q[c], s[y]);
+                    }
                 }
             }
             const bool more = t0 + kStride < hi;
@@ -570,6 +591,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_few_kernel(
                 typename F::Frag vt[KT];
                 value_terms(v, y, vt, lost_v);
                 mma_terms(vt, pt, o[y]);
+                if constexpr (KT == 3) __builtin_amdgcn_sched_barrier(0);
             }
             if (!more) break;
             load_v(un);
@@ -645,37 +667,85 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_few_kernel(
     }
 }
 
-// Joins the runs of a sequence that was split: row blockIdx.x, kv head
-// blockIdx.y, a thread four head dims of a column, the runs in order.
-__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a) {
+// Joins the runs of sequences that were split: rows blockIdx.x * each .. and
+// kv head blockIdx.y. A thread takes four head dims of a column and, where
+// that leaves threads, one of several shares of the runs; the shares are added
+// in order in LDS. A few rows a workgroup, so that a batch that was not split
+// costs one plan per workgroup of a grid the card holds at once (2048 rows of
+// 8 kv heads: 19 us with a workgroup for each, 4 so).
+__global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, int each) {
     const PagedArgs& p = a.p;
-    const int r = blockIdx.x, kvh = blockIdx.y, D = p.head_size;
-    const int seq = row_sequence(p, r);
-    if (seq < 0) return;
-    Found f;
+    __shared__ __attribute__((aligned(16))) float o_s[kThreads][4];
+    __shared__ float2 ml_s[kThreads];
+    const int kvh = blockIdx.y, D = p.head_size, tid = threadIdx.x;
     const float run = run_length(a);
-    if (!find(a, run, [&](int s, int, int) { return s == seq; }, f) || f.runs <= 1) return;
-    for (int x = threadIdx.x; x < p.group * (D / 4); x += kThreads) {
-        const int h = x / (D / 4), d = x % (D / 4) * 4;
-        const int cc = (r - f.w.row0) * p.group + h, tile = cc / kCols, c = cc % kCols;
-        const int step = f.w.tiles * p.n_kv_heads;
-        const std::size_t u0 = f.unit0 + (f.w.tiles - 1 - tile) * p.n_kv_heads + kvh;
-        float m = -INFINITY;
-        for (int y = 0; y < f.runs; ++y)
-            m = fmaxf(m, a.part_ml[(u0 + static_cast<std::size_t>(y) * step) * kCols + c].x);
-        float l = 0.0f;
-        floatx4 sum{0.f, 0.f, 0.f, 0.f};
-        for (int y = 0; y < f.runs; ++y) {
-            const std::size_t pc = (u0 + static_cast<std::size_t>(y) * step) * kCols + c;
-            const float2 ml = a.part_ml[pc];
-            const float fac = ml.x == m || ml.y != ml.y ? 1.0f
-                              : ml.x == -INFINITY       ? 0.0f
-                                                        : __builtin_amdgcn_exp2f(ml.x - m);
-            l += fac * ml.y;
-            sum += fac * *reinterpret_cast<const floatx4*>(a.part_o + pc * D + d);
+    const int last = min(p.rows, (static_cast<int>(blockIdx.x) + 1) * each);
+    for (int r = blockIdx.x * each; r < last;) {
+        const int seq = row_sequence(p, r);
+        if (seq < 0) {
+            ++r;
+            continue;
         }
-        float* dst = a.out + r * a.out_stride + (kvh * p.group + h) * D + d;
-        *reinterpret_cast<floatx4*>(dst) = l == 0.0f ? floatx4{0.f, 0.f, 0.f, 0.f} : sum * (1.0f / l);
+        Found f;
+        if (!find(a, run, [&](int s, int, int) { return s == seq; }, f) || f.w.n == 0) return;
+        const int stop = min(last, f.w.row0 + f.w.n);
+        if (f.runs <= 1) {
+            r = stop;
+            continue;
+        }
+        const int step = f.w.tiles * p.n_kv_heads, units = p.group * (D / 4);
+        const int width = min(units, kThreads), shares = kThreads / width;
+        const int share = tid / width;
+        for (; r < stop; ++r) {
+            for (int x0 = 0; x0 < units; x0 += width) {
+                const int x = x0 + tid % width;
+                const bool in = share < shares && x < units;
+                const int h = x / (D / 4), d = x % (D / 4) * 4;
+                const int cc = (r - f.w.row0) * p.group + h, tile = cc / kCols;
+                float m = -INFINITY, l = 0.0f;
+                floatx4 sum{0.f, 0.f, 0.f, 0.f};
+                auto add = [&](float2 ml, floatx4 o) {
+                    // A run whose sum is NaN has no maximum to go by.
+                    const float mn = fmaxf(m, ml.x);
+                    const float old = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+                    const float fac = ml.x == mn || ml.y != ml.y ? 1.0f
+                                      : ml.x == -INFINITY        ? 0.0f
+                                                                 : __builtin_amdgcn_exp2f(ml.x - mn);
+                    l = l * old + fac * ml.y;
+                    sum = sum * old + fac * o;
+                    m = mn;
+                };
+                if (in) {
+                    const std::size_t u0 = f.unit0 + (f.w.tiles - 1 - tile) * p.n_kv_heads + kvh;
+                    for (int y = share; y < f.runs; y += 4 * shares) {
+                        float2 ml[4];
+                        floatx4 o[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const std::size_t run_i = min(y + i * shares, f.runs - 1);
+                            const std::size_t pc = (u0 + run_i * step) * kCols + cc % kCols;
+                            ml[i] = a.part_ml[pc];
+                            o[i] = *reinterpret_cast<const floatx4*>(a.part_o + pc * D + d);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (y + i * shares < f.runs) add(ml[i], o[i]);
+                    }
+                }
+                if (shares > 1) {
+                    __syncthreads();
+                    ml_s[tid] = make_float2(m, l);
+                    *reinterpret_cast<floatx4*>(o_s[tid]) = sum;
+                    __syncthreads();
+                    if (share == 0)
+                        for (int y = 1; y < shares; ++y)
+                            add(ml_s[y * width + tid], *reinterpret_cast<const floatx4*>(o_s[y * width + tid]));
+                }
+                if (in && share == 0)
+                    *reinterpret_cast<floatx4*>(a.out + r * a.out_stride + (kvh * p.group + h) * D + d) =
+                        l == 0.0f ? floatx4{0.f, 0.f, 0.f, 0.f} : sum * (1.0f / l);
+            }
+        }
     }
 }
 
@@ -731,9 +801,12 @@ void run_paged_attention(PagedAttnArgs a, const em_paged_shape& s, float* scratc
         launch_few<_Float16>(a, grid, stream);
     else
         launch_few<__bf16>(a, grid, stream);
-    if (a.part_units)
-        hipLaunchKernelGGL(paged_join_kernel, dim3(a.p.rows, a.p.n_kv_heads), dim3(kThreads), 0,
-                           stream, a);
+    if (a.part_units) {
+        const int each = static_cast<int>(std::max(
+            1LL, static_cast<long long>(a.p.rows) * a.p.n_kv_heads / (4 * cu_count())));
+        hipLaunchKernelGGL(paged_join_kernel, dim3(ceil_div(a.p.rows, each), a.p.n_kv_heads),
+                           dim3(kThreads), 0, stream, a, each);
+    }
 }
 
 bool a16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
