@@ -24,7 +24,10 @@ namespace {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kCols = 16;       // columns of an item
+constexpr int kCols = 16;       // columns of a narrow item, and of a unit of partials
+constexpr int kWideCols = 128;  // columns of a wide one
+// Sequences of more columns than this take wide items.
+constexpr int kNarrowMost = 48;
 constexpr int kStep = 32;       // positions a wave takes at a time
 constexpr int kWaves = 4;
 constexpr int kMinRun = 128;    // positions of an item at least: one step a wave
@@ -38,6 +41,7 @@ struct PagedAttnArgs {
     long long q_stride, out_stride;
     float scale2;  // scale times log2 e: weights are 2^(x - max)
     int window;
+    int wide;       // sequences may take wide items
     int slots;      // workgroups to spread the positions over
     float* part_o;  // [unit][16 columns][head_size], a unit an item's 16 columns
     float2* part_ml;
@@ -51,7 +55,7 @@ struct SeqWork {
     int row0, n;         // its rows
     int p0;              // position of the first of them
     int first, end;      // positions that any row sees
-    int tiles;           // column tiles a kv head
+    int width, tiles;    // columns of a tile; tiles of a kv head
     __device__ int span() const { return max(1, end - first); }
 };
 
@@ -66,7 +70,8 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s) {
     w.p0 = len - w.n;
     w.end = min(max(len, 0), cap);
     w.first = a.window ? min(w.end, max(0, w.p0 + 1 - a.window)) : 0;
-    w.tiles = (w.n * p.group + kCols - 1) / kCols;
+    w.width = a.wide && w.n * p.group > kNarrowMost ? kWideCols : kCols;
+    w.tiles = (w.n * p.group + w.width - 1) / w.width;
     return w;
 }
 
@@ -130,7 +135,7 @@ __device__ __forceinline__ bool find(const PagedAttnArgs& a, float run, Hit hit,
         }
         // Units by the runs wanted; a sequence that would pass the partials'
         // memory stays whole (its units stay counted: all after it do too).
-        const int want = runs > 1 ? cells * runs : 0;
+        const int want = runs > 1 ? cells * runs * (w.width / kCols) : 0;
         const int ahead = units + wave_scan_int(want) - want;
         if (ahead + want > a.part_units) runs = min(runs, 1);
         const int mine = cells * runs;
@@ -147,6 +152,7 @@ __device__ __forceinline__ bool find(const PagedAttnArgs& a, float run, Hit hit,
             f.w.p0 = __shfl(w.p0, src, kWave);
             f.w.first = __shfl(w.first, src, kWave);
             f.w.end = __shfl(w.end, src, kWave);
+            f.w.width = __shfl(w.width, src, kWave);
             f.w.tiles = __shfl(w.tiles, src, kWave);
             return true;
         }
@@ -189,11 +195,18 @@ struct Ops<_Float16> {
     static constexpr float kWeight = 16384.0f;
 };
 
-__device__ __forceinline__ floatx4 mma16(f16x8 a, f16x8 b, floatx4 c) {
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ floatx4 mma(f16x8 a, f16x8 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ floatx4 mma16(bf16x8 a, bf16x8 b, floatx4 c) {
+__device__ __forceinline__ floatx4 mma(bf16x8 a, bf16x8 b, floatx4 c) {
     return mfma16x16x32(a, b, c);
+}
+__device__ __forceinline__ floatx16 mma(f16x8 a, f16x8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16 mma(bf16x8 a, bf16x8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
 // Eight fp32 values as terms. lost: as split3x8's (bf16).
@@ -243,19 +256,19 @@ __device__ __forceinline__ uint32_t word(const uint4& x, int i) {
 }
 
 // d += A x B over the pairs of terms kept.
-template <class F, int NT>
-__device__ __forceinline__ void mma_terms(const F (&k)[1], const F (&q)[NT], floatx4& d) {
+template <class F, int NT, class D>
+__device__ __forceinline__ void mma_terms(const F (&k)[1], const F (&q)[NT], D& d) {
 #pragma unroll
-    for (int t = NT - 1; t >= 0; --t) d = mma16(k[0], q[t], d);
+    for (int t = NT - 1; t >= 0; --t) d = mma(k[0], q[t], d);
 }
-template <class F>
-__device__ __forceinline__ void mma_terms(const F (&k)[3], const F (&q)[3], floatx4& d) {
-    d = mma16(k[2], q[0], d);
-    d = mma16(k[1], q[1], d);
-    d = mma16(k[0], q[2], d);
-    d = mma16(k[1], q[0], d);
-    d = mma16(k[0], q[1], d);
-    d = mma16(k[0], q[0], d);
+template <class F, class D>
+__device__ __forceinline__ void mma_terms(const F (&k)[3], const F (&q)[3], D& d) {
+    d = mma(k[2], q[0], d);
+    d = mma(k[1], q[1], d);
+    d = mma(k[0], q[2], d);
+    d = mma(k[1], q[0], d);
+    d = mma(k[0], q[1], d);
+    d = mma(k[0], q[0], d);
 }
 
 // --- one column, plainly ------------------------------------------------------------
@@ -341,6 +354,9 @@ struct Few {
     using O = Ops<T>;
     using Frag = typename O::Frag;
     static constexpr int NT = O::kTerms, KT = O::kCacheTerms;
+    static constexpr int kQueryAt = kWaves * kCols * ((DP + 4) * 4 + 8);
+    static constexpr bool kQueryLds = NT == 3;
+    static constexpr int kLds = kQueryAt + (kQueryLds ? C * NT * kWave * 16 : 0);
 };
 
 // A 16-bit value operand: element u of eight positions.
@@ -373,42 +389,35 @@ __device__ __forceinline__ void key_terms(const Raw8<float>& k, F (&t)[3]) {
     split_terms(k.v, t, lost);
 }
 
+// An item of the plan: columns [col0, col0 + cols) of kv head kvh of the
+// found sequence over positions [lo, hi), its partials' first unit.
+struct Item {
+    Found f;
+    int kvh, col0, cols, lo, hi, unit;
+};
+
 template <class T, int DP>
-__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_few_kernel(PagedAttnArgs a) {
+__device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& it, char* smem) {
     using F = Few<T, DP>;
     constexpr int C = F::C, VU = F::VU, NV = F::NV, NT = F::NT, KT = F::KT;
     constexpr int kRow = DP + 4;  // floats of a column in LDS
-    __shared__ __attribute__((aligned(16))) float o_s[kWaves][kCols][kRow];
-    __shared__ float2 ml_s[kWaves][kCols];
-    // fp32 keys and values take the registers that the query terms, the same
-    // in every wave, would need (148 spilled): those are read from LDS.
-    constexpr bool kQueryLds = KT == 3;
-    __shared__ __attribute__((aligned(16))) typename F::Frag q_s[kQueryLds ? C * NT * kWave : 1];
+    // The waves' outputs; before them the query terms of fp32 caches, whose
+    // keys and values take the registers (148 spilled with them): they are the
+    // same in every wave.
+    auto* o_s = reinterpret_cast<float(*)[kCols][kRow]>(smem);
+    auto* ml_s = reinterpret_cast<float2(*)[kCols]>(smem + sizeof(float) * kWaves * kCols * kRow);
+    constexpr bool kQueryLds = F::kQueryLds;
+    auto* q_s = reinterpret_cast<typename F::Frag*>(smem + F::kQueryAt);
     const PagedArgs& p = a.p;
     const int tid = threadIdx.x, lane = tid % kWave, g = lane >> 4, j = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const int D = p.head_size, item = blockIdx.x;
-
-    Found f;
-    const float run = run_length(a);
-    if (!find(a, run, [&](int, int before, int mine) { return item >= before && item < before + mine; },
-              f))
-        return;
-    // Item order in a sequence: kv heads fastest (the XCDs take blocks in
-    // turn, so a kv head's tiles share an L2), the longest tiles first.
-    const int at = item - f.item0, kvh = at % p.n_kv_heads;
-    const int tile = f.w.tiles - 1 - at / p.n_kv_heads % f.w.tiles;
-    const int part = at / p.n_kv_heads / f.w.tiles;
-    const int cols = min(kCols, f.w.n * p.group - tile * kCols);
-    const int col = tile * kCols + min(j, cols - 1);
+    const int D = p.head_size;
+    const Found& f = it.f;
+    const int kvh = it.kvh, cols = it.cols, lo = it.lo, hi = it.hi;
+    const int col = it.col0 + min(j, cols - 1);
     const int i = col / p.group, row = f.w.row0 + i, head = kvh * p.group + col % p.group;
     const int pq = f.w.p0 + i;
-    // The tile's positions, this item's run of them.
-    const int i0 = tile * kCols / p.group, i1 = (tile * kCols + cols - 1) / p.group;
-    const int first = max(f.w.first, a.window ? f.w.p0 + i0 + 1 - a.window : 0);
-    const int end = min(f.w.end, f.w.p0 + i1 + 1);
-    const int len = ((max(0, end - first) + f.runs - 1) / f.runs + kStep - 1) / kStep * kStep;
-    const int lo = first + part * len, hi = min(end, lo + len);
+    const int i0 = it.col0 / p.group, i1 = (it.col0 + cols - 1) / p.group;
     // Every column sees positions [all_lo, all_hi].
     const int all_lo = a.window ? f.w.p0 + i1 + 1 - a.window : 0, all_hi = f.w.p0 + i0;
 
@@ -534,7 +543,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_few_kernel(
                         for (int t = 0; t < NT; ++t) qt[t] = q_s[(c * NT + t) * kWave + lane];
                         mma_terms(kt, qt, s[y]);
                         // One split's terms at a time, not all of them in registers.
-                        __builtin_amdgcn_sched_barrier(0);
+                        if constexpr (KT == 3) __builtin_amdgcn_sched_barrier(0);
                     } else {
                         mma_terms(kt, q[c], s[y]);
                     }
@@ -637,7 +646,6 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_few_kernel(
     __syncthreads();
 
     // The four waves' sums, in wave order.
-    const int unit = f.unit0 + at;
     for (int x = tid; x < cols * (D / 4); x += kThreads) {
         const int c = x / (D / 4), d = x % (D / 4) * 4;
         float mm = -INFINITY, ll = 0.0f;
@@ -654,9 +662,9 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_few_kernel(
             ll += fac * ml.y;
             sum += fac * *reinterpret_cast<const floatx4*>(&o_s[y][c][d]);
         }
-        const int cc = tile * kCols + c;
+        const int cc = it.col0 + c;
         if (f.runs > 1) {
-            const std::size_t pc = static_cast<std::size_t>(unit) * kCols + c;
+            const std::size_t pc = static_cast<std::size_t>(it.unit) * kCols + c;
             *reinterpret_cast<floatx4*>(a.part_o + pc * D + d) = sum;
             if (d == 0) a.part_ml[pc] = make_float2(mm, ll);
         } else {
@@ -665,6 +673,369 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_few_kernel(
             *reinterpret_cast<floatx4*>(dst) = ll == 0.0f ? floatx4{0.f, 0.f, 0.f, 0.f} : sum * (1.0f / ll);
         }
     }
+}
+
+// --- 128 columns --------------------------------------------------------------------
+
+// A wide item: 128 columns, 32 a wave, over positions [lo, hi), 32 at a time
+// staged in LDS for the four waves. In lane (h, j), h = lane / 32:
+//  * S^T = K Q^T, 32 positions x 32 columns: the keys from LDS, Q's terms from
+//    registers (of three the last from LDS: with all in registers two
+//    workgroups a CU do not fit). The 16-byte units of a key's row are permuted
+//    by the key, so that 16 keys' reads of one unit fall into different banks.
+//  * The lane ends with column j's scores at positions 8 (r / 4) + 4h + r % 4,
+//    r < 16: per 16 positions the k values of O^T += V^T P^T, for which V's
+//    operand takes the positions in that order, DP / 32 head dims of eight
+//    positions read from LDS and put together by byte permutes.
+//  * O^T: column j, head dims DP / 32 (8 (r / 4) + 4h + r % 4) + u.
+// The next 32 positions are loaded into registers beside the products and
+// written to LDS after them (fp32: split into its three terms there). Bound by
+// the matrix cores, three products a multiply-add for bf16 and six for fp32,
+// beside the softmax of the other workgroup on the CU.
+template <class T, int DP>
+struct Wide {
+    using O = Ops<T>;
+    using Frag = typename O::Frag;
+    static constexpr int NT = O::kTerms, KT = O::kCacheTerms;
+    static constexpr int C = DP / 16, DU = DP / 32;  // k steps of S; head dims a lane
+    static constexpr int kRowBytes = DP * 2, kPlane = kStep * kRowBytes;
+    static constexpr int kStage = 2 * KT * kPlane;  // keys' planes, then values'
+    static constexpr int kBufs = 2 * kStage <= 64 * 1024 || KT == 3 ? (KT == 3 && DP > 64 ? 1 : 2) : 1;
+    static constexpr bool kQueryLds = NT == 3 && DP <= 128;
+    static constexpr int kQueryAt = kBufs * kStage;
+    static constexpr int kLds = kQueryAt + (kQueryLds ? kWaves * C * kWave * 16 : 0);
+    static constexpr int kLoads = kStep * (DP / 8) / kThreads;  // units a thread, of K and of V
+};
+
+// DU elements (DU / 2 words) of a value row for eight positions, and operand u.
+template <int DU>
+struct ValueRun {
+    uint32_t x[DU / 2];
+};
+
+template <class T, int DP>
+__device__ __forceinline__ void wide_item(const PagedAttnArgs& a, const Item& it, char* smem) {
+    using W = Wide<T, DP>;
+    using Frag = typename W::Frag;
+    constexpr int NT = W::NT, KT = W::KT, C = W::C, DU = W::DU, L = W::kLoads;
+    constexpr int NQ = W::kQueryLds ? 2 : NT;  // terms in registers
+    const PagedArgs& p = a.p;
+    const Found& f = it.f;
+    const int tid = threadIdx.x, lane = tid % kWave, h = lane >> 5, j = lane & 31;
+    const int w = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int D = p.head_size, kvh = it.kvh, lo = it.lo, hi = it.hi;
+    const int wc = 32 * w;  // the wave's first column in the tile
+    const bool idle = wc >= it.cols;
+    const int cin = min(wc + j, it.cols - 1), col = it.col0 + cin;
+    const int i = col / p.group, row = f.w.row0 + i, head = kvh * p.group + col % p.group;
+    const int pq = f.w.p0 + i;
+    // The wave's first and last row.
+    const int i0 = (it.col0 + min(wc, it.cols - 1)) / p.group;
+    const int i1 = (it.col0 + min(wc + 31, it.cols - 1)) / p.group;
+    const int all_lo = a.window ? f.w.p0 + i1 + 1 - a.window : 0, all_hi = f.w.p0 + i0;
+    const int wave_lo = a.window ? f.w.p0 + i0 + 1 - a.window : 0, wave_hi = f.w.p0 + i1;
+    const T* kc = static_cast<const T*>(a.kc) + kvh * p.head_stride;
+    const T* vc = static_cast<const T*>(a.vc) + kvh * p.head_stride;
+    auto* q_s = reinterpret_cast<Frag*>(smem + W::kQueryAt) + w * C * kWave;
+
+    // Head dims past the head size stay zero.
+    if (D < DP)
+        for (int x = tid; x < W::kBufs * W::kStage / 16; x += kThreads)
+            reinterpret_cast<uint4*>(smem)[x] = make_uint4(0, 0, 0, 0);
+
+    Frag q[C][NQ];
+    uint32_t lost_q = 0, lost_v = 0;
+    float top_q = 0.0f, unscale = 1.0f;
+    {
+        const float* src = a.q + row * a.q_stride + head * D;
+        auto load = [&](int c, float (&v)[8]) {
+            const int d = 16 * c + 8 * h;
+            const bool in = d < D;
+            const floatx4 x0 = *reinterpret_cast<const floatx4*>(src + (in ? d : 0));
+            const floatx4 x1 = *reinterpret_cast<const floatx4*>(src + (in ? d : 0) + 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = in ? x0[e] * a.scale2 : 0.0f;
+                v[4 + e] = in ? x1[e] * a.scale2 : 0.0f;
+            }
+        };
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float v[8];
+            load(c, v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top_q = fmaxf(top_q, fabsf(v[e]));
+            if constexpr (NT == 3) {
+                Frag t[3];
+                split_terms(v, t, lost_q);
+                q[c][0] = t[0];
+                q[c][1] = t[1];
+                if constexpr (W::kQueryLds)
+                    q_s[c * kWave + lane] = t[2];
+                else
+                    q[c][2] = t[2];
+            }
+        }
+        top_q = max32(top_q);
+        if constexpr (NT == 2) {
+            // To a largest value of 2^14 .. 2^15.
+            const int ex = top_q > 0.0f && top_q < INFINITY ? min(120, 14 - ilogbf(top_q)) : 0;
+            const float up = ldexpf(1.0f, ex);
+            unscale = ldexpf(1.0f, -ex);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                float v[8];
+                load(c, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] *= up;
+                split_terms(v, q[c], lost_q);
+            }
+        }
+    }
+    bool bad = KT == 3   ? (lost_q & 0xffffu) != 0 || !(top_q < 0x1p90f)
+               : NT == 3 ? (lost_q & 0xffffu) != 0
+                         : top_q != 0.0f && !(top_q >= 0x1p-100f && top_q < INFINITY);
+
+    // Unit x = tid + 256 y of a stage: position x / (DP / 8), head dims 8 (x % (DP / 8)).
+    constexpr int UR = DP / 8;
+    Raw8<T> kr[L], vr[L];
+    auto load = [&](uint32_t units) {
+#pragma unroll
+        for (int y = 0; y < L; ++y) {
+            const int x = tid + kThreads * y, c = x % UR;
+            const uint32_t u = __shfl(units, x / UR, kWave);
+            if (8 * c < D) {
+                const std::size_t at = static_cast<std::size_t>(u == kNoSlot ? 0 : u) * 8 + 8 * c;
+                kr[y].load(kc + at);
+                vr[y].load(vc + at);
+            }
+        }
+    };
+    auto permuted = [](int key, int c) {
+        return c ^ (DP == 64 ? (key >> 1) & 7 : key & 15);
+    };
+    auto store = [&](uint32_t there, char* buf) {
+#pragma unroll
+        for (int y = 0; y < L; ++y) {
+            const int x = tid + kThreads * y, c = x % UR, key = x / UR;
+            if (8 * c < D) {
+                if (!(there >> key & 1)) vr[y].zero();
+                char* kd = buf + key * W::kRowBytes + permuted(key, c) * 16;
+                char* vd = buf + KT * W::kPlane + key * W::kRowBytes + c * 16;
+                Frag t[KT];
+                key_terms(kr[y], t);
+#pragma unroll
+                for (int n = 0; n < KT; ++n) *reinterpret_cast<Frag*>(kd + n * W::kPlane) = t[n];
+                if constexpr (KT == 3)
+                    split_terms(vr[y].v, t, lost_v);
+                else
+                    key_terms(vr[y], t);
+#pragma unroll
+                for (int n = 0; n < KT; ++n) *reinterpret_cast<Frag*>(vd + n * W::kPlane) = t[n];
+            }
+        }
+    };
+    // Lane l holds the slot of position t0 + l % 32; the stage's positions that
+    // are there.
+    auto look = [&](int t0) {
+        const int t = t0 + j;
+        return t < hi ? slot_unit(p, f.seq, t) : kNoSlot;
+    };
+    auto mask = [](uint32_t units) { return static_cast<uint32_t>(__ballot(units != kNoSlot)); };
+
+    float m = -INFINITY, l = 0.0f;
+    floatx16 o[DU];
+#pragma unroll
+    for (int u = 0; u < DU; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[u][r] = 0.0f;
+
+    auto use = [&](int t0, uint32_t there, const char* buf) {
+        floatx16 s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            Frag k[KT], qt[NT];
+#pragma unroll
+            for (int n = 0; n < KT; ++n)
+                k[n] = *reinterpret_cast<const Frag*>(buf + n * W::kPlane + j * W::kRowBytes +
+                                                      permuted(j, 2 * c + h) * 16);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) qt[n] = q[c][n];
+            if constexpr (W::kQueryLds) qt[2] = q_s[c * kWave + lane];
+            mma_terms(k, qt, s);
+        }
+        if constexpr (NT == 2) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] *= unscale;
+        }
+        if (there != 0xffffffffu || t0 < all_lo || t0 + kStep - 1 > all_hi) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int x = 8 * (r / 4) + 4 * h + r % 4, t = t0 + x;
+                const bool seen = (there >> x & 1) && t <= pq && !(a.window && t <= pq - a.window);
+                s[r] = seen ? s[r] : -INFINITY;
+            }
+        }
+        float mb = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mb = fmaxf(mb, s[r]);
+        const float mn = fmaxf(m, max32(mb));
+        if (__ballot(mn > m)) {
+            const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= alpha;
+#pragma unroll
+            for (int u = 0; u < DU; ++u) o[u] *= alpha;
+            m = mn;
+        }
+        const float base = mn == -INFINITY ? 0.0f : mn;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            float pw[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                pw[e] = __builtin_amdgcn_exp2f(s[8 * y + e] - base);
+                l += pw[e];
+                pw[e] *= W::O::kWeight;
+            }
+            Frag pt[NT];
+            uint32_t lost_p = 0;
+            split_terms(pw, pt, lost_p);
+            // A plane at a time, the smallest first.
+#pragma unroll
+            for (int n = KT - 1; n >= 0; --n) {
+                ValueRun<DU> v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    v[e] = *reinterpret_cast<const ValueRun<DU>*>(
+                        buf + (KT + n) * W::kPlane +
+                        (16 * y + 4 * h + (e < 4 ? e : 4 + e)) * W::kRowBytes + j * DU * 2);
+#pragma unroll
+                for (int u = 0; u < DU; ++u) {
+                    const uint32_t sel = u & 1 ? 0x07060302u : 0x05040100u;
+                    uint4 x;
+                    x.x = __builtin_amdgcn_perm(v[1].x[u / 2], v[0].x[u / 2], sel);
+                    x.y = __builtin_amdgcn_perm(v[3].x[u / 2], v[2].x[u / 2], sel);
+                    x.z = __builtin_amdgcn_perm(v[5].x[u / 2], v[4].x[u / 2], sel);
+                    x.w = __builtin_amdgcn_perm(v[7].x[u / 2], v[6].x[u / 2], sel);
+                    const Frag vt = __builtin_bit_cast(Frag, x);
+#pragma unroll
+                    for (int t = NT - 1 - n; t >= 0; --t) o[u] = mma(vt, pt[t], o[u]);
+                }
+            }
+        }
+    };
+
+    if (lo < hi) {
+        uint32_t units = look(lo), next = look(lo + kStep);
+        if (D < DP) __syncthreads();  // the zeros
+        load(units);
+        store(mask(units), smem);
+        for (int t0 = lo, s = 0; t0 < hi; t0 += kStep, ++s) {
+            char* buf = smem + (W::kBufs == 2 ? (s & 1) * W::kStage : 0);
+            __syncthreads();  // this stage is in LDS, the one before has been read
+            const bool more = t0 + kStep < hi;
+            const uint32_t there = mask(units);
+            units = next;
+            if (more) load(units);
+            next = look(t0 + 2 * kStep);
+            if (!idle && t0 <= wave_hi && t0 + kStep > wave_lo) use(t0, there, buf);
+            if (W::kBufs == 1) __syncthreads();
+            if (more) store(mask(units), smem + (W::kBufs == 2 ? ((s + 1) & 1) * W::kStage : 0));
+        }
+    }
+    // Whether any wave stored a value that dropped bits.
+    bool v_lost = false;
+    if constexpr (KT == 3) {
+        auto* flag = reinterpret_cast<int*>(smem);
+        __syncthreads();
+        if (tid == 0) *flag = 0;
+        __syncthreads();
+        if (lost_v & 0xffffu) *flag = 1;
+        __syncthreads();
+        v_lost = *flag != 0;
+    }
+    if (idle) return;
+    l = sum32(l);
+    float low = INFINITY;
+#pragma unroll
+    for (int u = 0; u < DU; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int d = DU * (8 * (r / 4) + 4 * h + r % 4) + u;
+            const float x = fabsf(o[u][r]);
+            bad |= d < D && !(x < INFINITY);
+            low = d < D ? fminf(low, x) : low;
+        }
+    if constexpr (KT == 3) bad |= v_lost && low < 0x1p-50f;
+    bad |= !(l < INFINITY);
+    unsigned long long redo = __ballot(bad);
+    redo = (redo | redo >> 32) & 0xffffffffull;
+    const bool mine = wc + j < it.cols;
+    const std::size_t pc = static_cast<std::size_t>(it.unit) * kCols + cin;
+    float* dst = f.runs > 1 ? a.part_o + pc * D : a.out + row * a.out_stride + head * D;
+    const float by = (f.runs > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l) * (1.0f / W::O::kWeight);
+    if (mine && !(redo >> j & 1)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int d = DU * (8 * (r / 4) + 4 * h + r % 4);
+#pragma unroll
+            for (int u = 0; u < DU; u += 2)
+                if (d + u < D)
+                    *reinterpret_cast<float2*>(dst + d + u) = make_float2(o[u][r] * by, o[u + 1][r] * by);
+        }
+        if (f.runs > 1 && h == 0) a.part_ml[pc] = make_float2(m, l);
+    }
+    while (redo) {
+        const int c = __ffsll(redo) - 1;
+        redo &= redo - 1;
+        if (wc + c >= it.cols) break;
+        float po[DP / kWave], pm, pl;
+        const int prow = __shfl(row, c, kWave), phead = __shfl(head, c, kWave);
+        plain_column<T, DP / kWave>(a, f.seq, prow, phead, __shfl(pq, c, kWave), lo, hi, kStep, pm, pl, po);
+        const std::size_t ppc = static_cast<std::size_t>(it.unit) * kCols + wc + c;
+        float* pdst = f.runs > 1 ? a.part_o + ppc * D : a.out + prow * a.out_stride + phead * D;
+        const float pby = f.runs > 1 ? 1.0f : pl == 0.0f ? 0.0f : 1.0f / pl;
+#pragma unroll
+        for (int n = 0; n < DP / kWave; ++n)
+            if (lane + kWave * n < D) pdst[lane + kWave * n] = po[n] * pby;
+        if (f.runs > 1 && lane == 0) a.part_ml[ppc] = make_float2(pm, pl);
+    }
+}
+
+// WIDE: for calls in which a sequence may have more than kNarrowMost columns.
+template <class T, int DP, bool WIDE>
+__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attn_kernel(PagedAttnArgs a) {
+    constexpr int kNarrowLds = Few<T, DP>::kLds, kWideLds = Wide<T, DP>::kLds;
+    __shared__ __attribute__((aligned(16))) char smem[WIDE && kWideLds > kNarrowLds ? kWideLds : kNarrowLds];
+    const PagedArgs& p = a.p;
+    const int item = blockIdx.x;
+    Item it;
+    const float run = run_length(a);
+    if (!find(a, run, [&](int, int before, int mine) { return item >= before && item < before + mine; },
+              it.f))
+        return;
+    // Item order in a sequence: kv heads fastest (the XCDs take blocks in
+    // turn, so a kv head's tiles share an L2), the longest tiles first.
+    const SeqWork& w = it.f.w;
+    const int at = item - it.f.item0, tile = w.tiles - 1 - at / p.n_kv_heads % w.tiles;
+    it.kvh = at % p.n_kv_heads;
+    it.col0 = tile * w.width;
+    it.cols = min(w.width, w.n * p.group - it.col0);
+    it.unit = it.f.unit0 + at * (w.width / kCols);
+    // The tile's positions, this item's run of them.
+    const int i0 = it.col0 / p.group, i1 = (it.col0 + it.cols - 1) / p.group;
+    const int first = max(w.first, a.window ? w.p0 + i0 + 1 - a.window : 0);
+    const int end = min(w.end, w.p0 + i1 + 1);
+    const int len =
+        ((max(0, end - first) + it.f.runs - 1) / it.f.runs + kStep - 1) / kStep * kStep;
+    it.lo = first + at / p.n_kv_heads / w.tiles * len;
+    it.hi = min(end, it.lo + len);
+    if (WIDE && w.width == kWideCols)
+        wide_item<T, DP>(a, it, smem);
+    else
+        narrow_item<T, DP>(a, it, smem);
 }
 
 // Joins the runs of sequences that were split: rows blockIdx.x * each .. and
@@ -693,7 +1064,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, i
             r = stop;
             continue;
         }
-        const int step = f.w.tiles * p.n_kv_heads, units = p.group * (D / 4);
+        const int step = f.w.tiles * p.n_kv_heads * (f.w.width / kCols), units = p.group * (D / 4);
         const int width = min(units, kThreads), shares = kThreads / width;
         const int share = tid / width;
         for (; r < stop; ++r) {
@@ -701,7 +1072,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, i
                 const int x = x0 + tid % width;
                 const bool in = share < shares && x < units;
                 const int h = x / (D / 4), d = x % (D / 4) * 4;
-                const int cc = (r - f.w.row0) * p.group + h, tile = cc / kCols;
+                const int cc = (r - f.w.row0) * p.group + h, tile = cc / f.w.width;
                 float m = -INFINITY, l = 0.0f;
                 floatx4 sum{0.f, 0.f, 0.f, 0.f};
                 auto add = [&](float2 ml, floatx4 o) {
@@ -716,7 +1087,9 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, i
                     m = mn;
                 };
                 if (in) {
-                    const std::size_t u0 = f.unit0 + (f.w.tiles - 1 - tile) * p.n_kv_heads + kvh;
+                    const int of = f.w.width / kCols;  // units of an item
+                    const std::size_t u0 = f.unit0 + ((f.w.tiles - 1 - tile) * p.n_kv_heads + kvh) * of +
+                                           cc % f.w.width / kCols;
                     for (int y = share; y < f.runs; y += 4 * shares) {
                         float2 ml[4];
                         floatx4 o[4];
@@ -759,48 +1132,74 @@ bool can_split(const em_paged_shape& s) {
     return static_cast<long long>(s.page_size) * s.max_pages >= kMinRun * 3 / 2;
 }
 
+// Whether a sequence of the call may take wide items.
+bool can_widen(const em_paged_shape& s, std::size_t rows) {
+    return rows * static_cast<std::size_t>(s.n_heads / s.n_kv_heads) >
+           static_cast<std::size_t>(kNarrowMost);
+}
+
 // Units of partials at most. A sequence of two runs or more has them over 1.5
 // lengths or more, so runs <= 4/3 positions / length, and all columns'
 // positions / length is at most the slots; one sixteenth is added for the
 // float arithmetic of the plan.
-int partial_units(const em_paged_shape& s) {
-    return can_split(s) ? paged_slots() * 17 / 12 + 1 : 0;
+int partial_units(const em_paged_shape& s, std::size_t rows) {
+    if (!can_split(s)) return 0;
+    return (paged_slots() * 17 / 12 + 1) * (can_widen(s, rows) ? kWideCols / kCols : 1);
 }
 
-std::size_t paged_attention_scratch(const em_paged_shape& s, std::size_t, std::size_t) {
-    return static_cast<std::size_t>(partial_units(s)) * kCols *
+std::size_t paged_attention_scratch(const em_paged_shape& s, std::size_t, std::size_t rows) {
+    return static_cast<std::size_t>(partial_units(s, rows)) * kCols *
            (static_cast<std::size_t>(s.head_size) + 2);
 }
 
-template <class T>
-void launch_few(const PagedAttnArgs& a, dim3 grid, hipStream_t stream) {
-    if (a.p.head_size <= 64)
-        hipLaunchKernelGGL((paged_few_kernel<T, 64>), grid, dim3(kThreads), 0, stream, a);
-    else if (a.p.head_size <= 128)
-        hipLaunchKernelGGL((paged_few_kernel<T, 128>), grid, dim3(kThreads), 0, stream, a);
+// Items at most: column tiles (each sequence's last may be partly full;
+// narrow ones and wide), and a run more for each run length in all columns'
+// positions.
+long long paged_items(const em_paged_shape& s, long long n_seqs, long long rows) {
+    const long long cols = rows * (s.n_heads / s.n_kv_heads), seqs = std::min(n_seqs, rows);
+    const bool wide = can_widen(s, static_cast<std::size_t>(rows));
+    long long tiles = cols / kCols + seqs;
+    if (wide) {
+        tiles = std::min(tiles, seqs * (kNarrowMost / kCols));
+        tiles += cols / kWideCols + std::min(seqs, cols / (kNarrowMost + 1));
+    }
+    const int slots = paged_slots();
+    return tiles * s.n_kv_heads + (can_split(s) ? slots + slots / 16 + 1 : 0);
+}
+
+template <class T, int DP>
+void launch_attn(const PagedAttnArgs& a, dim3 grid, hipStream_t stream) {
+    if (a.wide)
+        hipLaunchKernelGGL((paged_attn_kernel<T, DP, true>), grid, dim3(kThreads), 0, stream, a);
     else
-        hipLaunchKernelGGL((paged_few_kernel<T, 256>), grid, dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL((paged_attn_kernel<T, DP, false>), grid, dim3(kThreads), 0, stream, a);
+}
+template <class T>
+void launch_attn(const PagedAttnArgs& a, dim3 grid, hipStream_t stream) {
+    if (a.p.head_size <= 64)
+        launch_attn<T, 64>(a, grid, stream);
+    else if (a.p.head_size <= 128)
+        launch_attn<T, 128>(a, grid, stream);
+    else
+        launch_attn<T, 256>(a, grid, stream);
 }
 
 void run_paged_attention(PagedAttnArgs a, const em_paged_shape& s, float* scratch,
                          hipStream_t stream) {
+    const auto rows = static_cast<std::size_t>(a.p.rows);
+    a.wide = can_widen(s, rows);
     a.slots = paged_slots();
-    a.part_units = partial_units(s);
+    a.part_units = partial_units(s, rows);
     a.part_o = scratch;
     a.part_ml = reinterpret_cast<float2*>(
         scratch + static_cast<std::size_t>(a.part_units) * kCols * s.head_size);
-    // Column tiles at most (each sequence's last may be partly full), a run
-    // more for each run length in all columns' positions.
-    const long long cols = static_cast<long long>(a.p.rows) * a.p.group;
-    const long long tiles = cols / kCols + std::min(a.p.n_seqs, a.p.rows);
-    const long long items = tiles * a.p.n_kv_heads + (a.part_units ? a.slots + a.slots / 16 + 1 : 0);
-    const dim3 grid(static_cast<unsigned>(items));
+    const dim3 grid(static_cast<unsigned>(paged_items(s, a.p.n_seqs, a.p.rows)));
     if (s.type == EM_CACHE_F32)
-        launch_few<float>(a, grid, stream);
+        launch_attn<float>(a, grid, stream);
     else if (s.type == EM_CACHE_F16)
-        launch_few<_Float16>(a, grid, stream);
+        launch_attn<_Float16>(a, grid, stream);
     else
-        launch_few<__bf16>(a, grid, stream);
+        launch_attn<__bf16>(a, grid, stream);
     if (a.part_units) {
         const int each = static_cast<int>(std::max(
             1LL, static_cast<long long>(a.p.rows) * a.p.n_kv_heads / (4 * cu_count())));
@@ -851,6 +1250,8 @@ int em_paged_attention(const em_paged_shape* s, const em_paged_batch* b, size_t 
         (need && !em::a16(scratch)))
         return fail(EM_EINVAL, "paged_attention: pointers must be 16-byte aligned");
     if (!em::device_present()) return fail(EM_ENODEV, "paged_attention: no usable GPU");
+    if (em::paged_items(*s, b->n_seqs, static_cast<long long>(rows)) >= (1LL << 24))
+        return fail(EM_EINVAL, "paged_attention: more rows and heads than one launch takes");
     try {
         em::PagedAttnArgs a{};
         a.p = em::paged_args(*s, *b, rows);
