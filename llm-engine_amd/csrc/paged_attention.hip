@@ -26,11 +26,13 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kCols = 16;       // columns of a narrow item, and of a unit of partials
 constexpr int kWideCols = 128;  // columns of a wide one
-// Sequences of more columns than this take wide items.
-constexpr int kNarrowMost = 48;
+// Sequences of more columns than this take wide items: us at 48 / 32 / 16, five
+// of 32 to 40 rows of 32 heads (fp32, 1456 positions) 193 / 125 / 126, 47 of 5 to
+// 6 rows of 24 heads on 8 (fp16, 4927 positions) 239 / 235 / 346.
+constexpr int kNarrowMost = 32;
 constexpr int kStep = 32;       // positions a wave takes at a time
 constexpr int kWaves = 4;
-constexpr int kMinRun = 128;    // positions of an item at least: one step a wave
+constexpr int kMinRun = 128;    // positions of a narrow item at least: one step a wave
 constexpr uint32_t kNoSlot = 0xffffffffu;
 
 struct PagedAttnArgs {
@@ -43,6 +45,7 @@ struct PagedAttnArgs {
     int window;
     int wide;       // sequences may take wide items
     int slots;      // workgroups to spread the positions over
+    int min_wide;   // positions of a wide item at least
     float* part_o;  // [unit][16 columns][head_size], a unit an item's 16 columns
     float2* part_ml;
     int part_units;
@@ -56,7 +59,7 @@ struct SeqWork {
     int p0;              // position of the first of them
     int first, end;      // positions that any row sees
     int width, tiles;    // columns of a tile; tiles of a kv head
-    __device__ int span() const { return max(1, end - first); }
+    int span;            // positions of a tile, at most
 };
 
 __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s) {
@@ -72,6 +75,8 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s) {
     w.first = a.window ? min(w.end, max(0, w.p0 + 1 - a.window)) : 0;
     w.width = a.wide && w.n * p.group > kNarrowMost ? kWideCols : kCols;
     w.tiles = (w.n * p.group + w.width - 1) / w.width;
+    w.span = max(1, w.end - w.first);
+    if (a.window) w.span = min(w.span, a.window + (w.width + p.group - 1) / p.group);
     return w;
 }
 
@@ -90,74 +95,89 @@ __device__ __forceinline__ int wave_scan_int(int v) {  // inclusive
     return v;
 }
 
-// A run's positions: all columns' positions over the slots.
-__device__ __forceinline__ float run_length(const PagedAttnArgs& a) {
+// All columns' positions over the slots. Narrow items take half of that where a
+// sequence would be only a few of them: rounding leaves items of up to one and
+// a half lengths, which twice as many even out (64 sequences of 500 to 4000
+// positions 167 / 146 us, 2 of 100000 189 / 195; a cut costs a wide item its
+// queries' terms again, 2048 rows at 8148 717 / 752).
+struct RunLength {
+    float narrow, wide;
+};
+__device__ __forceinline__ RunLength run_length(const PagedAttnArgs& a) {
     const int lane = threadIdx.x % kWave;
-    float total = 0.0f;
+    float total = 0.0f, tiles = 0.0f;
     for (int s0 = 0; s0 < a.p.n_seqs; s0 += kWave) {
-        float t = 0.0f;
+        float t = 0.0f, n = 0.0f;
         if (s0 + lane < a.p.n_seqs) {
             const SeqWork w = seq_work(a, s0 + lane);
-            t = static_cast<float>(w.tiles) * static_cast<float>(w.span());
+            n = static_cast<float>(w.tiles);
+            t = n * static_cast<float>(w.span);
         }
         total += wave_sum(t);
+        tiles += wave_sum(n);
     }
-    total *= static_cast<float>(a.p.n_kv_heads);
-    return fmaxf(static_cast<float>(kMinRun), total / static_cast<float>(a.slots));
+    const float kv = static_cast<float>(a.p.n_kv_heads), slots = static_cast<float>(a.slots);
+    const float run = total * kv / slots;
+    const float part = tiles * kv * 16.0f > slots ? 0.5f : 1.0f;
+    return {fmaxf(run * part, static_cast<float>(kMinRun)), fmaxf(run, static_cast<float>(a.min_wide))};
 }
 
-// Runs of a sequence: its positions over a run's length, rounded to nearest,
-// so that no item is longer than one and a half of them.
-__device__ __forceinline__ int runs_of(const SeqWork& w, float run) {
-    return max(1, min(1 << 16, static_cast<int>(static_cast<float>(w.span()) / run + 0.5f)));
+// Runs of a sequence: its positions over a run's length, to the nearest whole
+// number.
+__device__ __forceinline__ int runs_of(const SeqWork& w, const RunLength& run) {
+    const float n = static_cast<float>(w.span) / (w.width == kWideCols ? run.wide : run.narrow);
+    return max(1, min(1 << 16, static_cast<int>(n + 0.5f)));
 }
 
-// Finds by wave the sequence for which `hit(s, items before, items of it)`
-// holds, walking the running sums; `units` counts the partials' units
-// likewise (sequences of one run need none, and none is split past the
-// partials' memory).
+// Where a sequence's items and partials are. Items of wide sequences come
+// first: they take longest and the narrow ones fill in beside and behind them.
+// Sequences of one run need no partials, and none is split past the partials'
+// memory.
 struct Found {
     int seq, runs, item0, unit0;
     SeqWork w;
 };
+// By wave: the sequence for which hit(s, items before, items of it) holds.
 template <class Hit>
-__device__ __forceinline__ bool find(const PagedAttnArgs& a, float run, Hit hit, Found& f) {
+__device__ __forceinline__ bool find(const PagedAttnArgs& a, const RunLength& run, Hit hit, Found& f) {
     const int lane = threadIdx.x % kWave;
     int items = 0, units = 0;
-    for (int s0 = 0; s0 < a.p.n_seqs; s0 += kWave) {
-        const int s = s0 + lane;
-        SeqWork w{};
-        int cells = 0, runs = 0;
-        if (s < a.p.n_seqs) {
-            w = seq_work(a, s);
-            cells = w.tiles * a.p.n_kv_heads;
-            runs = runs_of(w, run);
+    for (int width = a.wide ? kWideCols : kCols; width; width = width == kWideCols ? kCols : 0) {
+        for (int s0 = 0; s0 < a.p.n_seqs; s0 += kWave) {
+            const int s = s0 + lane;
+            SeqWork w{};
+            int cells = 0, runs = 0;
+            if (s < a.p.n_seqs) {
+                w = seq_work(a, s);
+                if (w.width == width) cells = w.tiles * a.p.n_kv_heads;
+                runs = runs_of(w, run);
+            }
+            // Units by the runs wanted; a sequence that would pass the partials'
+            // memory stays whole (its units stay counted: all after it do too).
+            const int want = runs > 1 ? cells * runs * (width / kCols) : 0;
+            const int ahead = units + wave_scan_int(want) - want;
+            if (ahead + want > a.part_units) runs = min(runs, 1);
+            const int mine = cells * runs;
+            const int before = items + wave_scan_int(mine) - mine;
+            const unsigned long long got = __ballot(mine > 0 && hit(s, before, mine));
+            if (got) {
+                const int src = __ffsll(got) - 1;
+                f.seq = s0 + src;
+                f.runs = __shfl(runs, src, kWave);
+                f.item0 = __shfl(before, src, kWave);
+                f.unit0 = __shfl(ahead, src, kWave);
+                f.w.row0 = __shfl(w.row0, src, kWave);
+                f.w.n = __shfl(w.n, src, kWave);
+                f.w.p0 = __shfl(w.p0, src, kWave);
+                f.w.first = __shfl(w.first, src, kWave);
+                f.w.end = __shfl(w.end, src, kWave);
+                f.w.width = width;
+                f.w.tiles = __shfl(w.tiles, src, kWave);
+                return true;
+            }
+            items = __shfl(before + mine, kWave - 1, kWave);
+            units = __shfl(ahead + want, kWave - 1, kWave);
         }
-        // Units by the runs wanted; a sequence that would pass the partials'
-        // memory stays whole (its units stay counted: all after it do too).
-        const int want = runs > 1 ? cells * runs * (w.width / kCols) : 0;
-        const int ahead = units + wave_scan_int(want) - want;
-        if (ahead + want > a.part_units) runs = min(runs, 1);
-        const int mine = cells * runs;
-        const int before = items + wave_scan_int(mine) - mine;
-        const unsigned long long got = __ballot(s < a.p.n_seqs && hit(s, before, mine));
-        if (got) {
-            const int src = __ffsll(got) - 1;
-            f.seq = s0 + src;
-            f.runs = __shfl(runs, src, kWave);
-            f.item0 = __shfl(before, src, kWave);
-            f.unit0 = __shfl(ahead, src, kWave);
-            f.w.row0 = __shfl(w.row0, src, kWave);
-            f.w.n = __shfl(w.n, src, kWave);
-            f.w.p0 = __shfl(w.p0, src, kWave);
-            f.w.first = __shfl(w.first, src, kWave);
-            f.w.end = __shfl(w.end, src, kWave);
-            f.w.width = __shfl(w.width, src, kWave);
-            f.w.tiles = __shfl(w.tiles, src, kWave);
-            return true;
-        }
-        items = __shfl(before + mine, kWave - 1, kWave);
-        units = __shfl(ahead + want, kWave - 1, kWave);
     }
     return false;
 }
@@ -1012,7 +1032,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attn_kernel
     const PagedArgs& p = a.p;
     const int item = blockIdx.x;
     Item it;
-    const float run = run_length(a);
+    const RunLength run = run_length(a);
     if (!find(a, run, [&](int, int before, int mine) { return item >= before && item < before + mine; },
               it.f))
         return;
@@ -1039,18 +1059,20 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attn_kernel
 }
 
 // Joins the runs of sequences that were split: rows blockIdx.x * each .. and
-// kv head blockIdx.y. A thread takes four head dims of a column and, where
-// that leaves threads, one of several shares of the runs; the shares are added
-// in order in LDS. A few rows a workgroup, so that a batch that was not split
-// costs one plan per workgroup of a grid the card holds at once (2048 rows of
-// 8 kv heads: 19 us with a workgroup for each, 4 so).
+// kv head blockIdx.y. A thread takes four head dims of a column of one row;
+// where a row leaves threads, they take other rows, or shares of the runs where
+// there are many, which are added in order in LDS. Several rows a workgroup, so
+// that a batch that was not split costs one plan per workgroup of a grid that
+// the card holds at once (2048 rows of 8 kv heads: 19 us with a workgroup for
+// each, 4 so).
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, int each) {
     const PagedArgs& p = a.p;
     __shared__ __attribute__((aligned(16))) float o_s[kThreads][4];
     __shared__ float2 ml_s[kThreads];
     const int kvh = blockIdx.y, D = p.head_size, tid = threadIdx.x;
-    const float run = run_length(a);
+    const RunLength run = run_length(a);
     const int last = min(p.rows, (static_cast<int>(blockIdx.x) + 1) * each);
+    const int units = p.group * (D / 4), width = min(units, kThreads);
     for (int r = blockIdx.x * each; r < last;) {
         const int seq = row_sequence(p, r);
         if (seq < 0) {
@@ -1058,21 +1080,24 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, i
             continue;
         }
         Found f;
-        if (!find(a, run, [&](int s, int, int) { return s == seq; }, f) || f.w.n == 0) return;
+        if (!find(a, run, [&](int s, int, int) { return s == seq; }, f)) return;
         const int stop = min(last, f.w.row0 + f.w.n);
         if (f.runs <= 1) {
             r = stop;
             continue;
         }
-        const int step = f.w.tiles * p.n_kv_heads * (f.w.width / kCols), units = p.group * (D / 4);
-        const int width = min(units, kThreads), shares = kThreads / width;
-        const int share = tid / width;
-        for (; r < stop; ++r) {
+        const int of = f.w.width / kCols;  // units of an item
+        const int step = f.w.tiles * p.n_kv_heads * of;
+        const int shares = max(1, min(kThreads / width, f.runs / 8));
+        const int abreast = kThreads / (width * shares);  // rows at a time
+        const int share = tid / width % shares, mine = tid / (width * shares);
+        for (; r < stop; r += abreast) {
+            const int row = r + mine;
             for (int x0 = 0; x0 < units; x0 += width) {
                 const int x = x0 + tid % width;
-                const bool in = share < shares && x < units;
+                const bool in = mine < abreast && row < stop && x < units;
                 const int h = x / (D / 4), d = x % (D / 4) * 4;
-                const int cc = (r - f.w.row0) * p.group + h, tile = cc / f.w.width;
+                const int cc = (row - f.w.row0) * p.group + h, tile = cc / f.w.width;
                 float m = -INFINITY, l = 0.0f;
                 floatx4 sum{0.f, 0.f, 0.f, 0.f};
                 auto add = [&](float2 ml, floatx4 o) {
@@ -1087,7 +1112,6 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, i
                     m = mn;
                 };
                 if (in) {
-                    const int of = f.w.width / kCols;  // units of an item
                     const std::size_t u0 = f.unit0 + ((f.w.tiles - 1 - tile) * p.n_kv_heads + kvh) * of +
                                            cc % f.w.width / kCols;
                     for (int y = share; y < f.runs; y += 4 * shares) {
@@ -1110,15 +1134,16 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, i
                     ml_s[tid] = make_float2(m, l);
                     *reinterpret_cast<floatx4*>(o_s[tid]) = sum;
                     __syncthreads();
-                    if (share == 0)
+                    if (in && share == 0)
                         for (int y = 1; y < shares; ++y)
                             add(ml_s[y * width + tid], *reinterpret_cast<const floatx4*>(o_s[y * width + tid]));
                 }
                 if (in && share == 0)
-                    *reinterpret_cast<floatx4*>(a.out + r * a.out_stride + (kvh * p.group + h) * D + d) =
+                    *reinterpret_cast<floatx4*>(a.out + row * a.out_stride + (kvh * p.group + h) * D + d) =
                         l == 0.0f ? floatx4{0.f, 0.f, 0.f, 0.f} : sum * (1.0f / l);
             }
         }
+        r = stop;
     }
 }
 
@@ -1138,13 +1163,13 @@ bool can_widen(const em_paged_shape& s, std::size_t rows) {
            static_cast<std::size_t>(kNarrowMost);
 }
 
-// Units of partials at most. A sequence of two runs or more has them over 1.5
-// lengths or more, so runs <= 4/3 positions / length, and all columns'
-// positions / length is at most the slots; one sixteenth is added for the
-// float arithmetic of the plan.
+// Units of partials at most. All columns' positions over a run's length are at
+// most the slots. A wide sequence that is split has 1.5 lengths or more, so no
+// more than 4/3 runs a length; a narrow one twice that; one sixteenth is added
+// for the float arithmetic of the plan.
 int partial_units(const em_paged_shape& s, std::size_t rows) {
     if (!can_split(s)) return 0;
-    return (paged_slots() * 17 / 12 + 1) * (can_widen(s, rows) ? kWideCols / kCols : 1);
+    return (paged_slots() * 17 / 12 + 1) * (can_widen(s, rows) ? kWideCols / kCols : 2);
 }
 
 std::size_t paged_attention_scratch(const em_paged_shape& s, std::size_t, std::size_t rows) {
@@ -1153,8 +1178,8 @@ std::size_t paged_attention_scratch(const em_paged_shape& s, std::size_t, std::s
 }
 
 // Items at most: column tiles (each sequence's last may be partly full;
-// narrow ones and wide), and a run more for each run length in all columns'
-// positions.
+// narrow ones and wide), and up to two runs more for each run length in all
+// columns' positions.
 long long paged_items(const em_paged_shape& s, long long n_seqs, long long rows) {
     const long long cols = rows * (s.n_heads / s.n_kv_heads), seqs = std::min(n_seqs, rows);
     const bool wide = can_widen(s, static_cast<std::size_t>(rows));
@@ -1164,7 +1189,7 @@ long long paged_items(const em_paged_shape& s, long long n_seqs, long long rows)
         tiles += cols / kWideCols + std::min(seqs, cols / (kNarrowMost + 1));
     }
     const int slots = paged_slots();
-    return tiles * s.n_kv_heads + (can_split(s) ? slots + slots / 16 + 1 : 0);
+    return tiles * s.n_kv_heads + (can_split(s) ? 2 * slots + slots / 8 + 1 : 0);
 }
 
 template <class T, int DP>
@@ -1189,6 +1214,11 @@ void run_paged_attention(PagedAttnArgs a, const em_paged_shape& s, float* scratc
     const auto rows = static_cast<std::size_t>(a.p.rows);
     a.wide = can_widen(s, rows);
     a.slots = paged_slots();
+    // A stage of fp32 takes twice the products and both splits: us at 192 /
+    // 512 positions, three chunks of 200 rows of 8 heads of 64 (fp32) 45 / 62,
+    // one of 1205 rows of 24 heads of 96 85 / 116; eight of up to 466 rows of 20
+    // heads of 80 (fp16) 50 / 34.
+    a.min_wide = s.type == EM_CACHE_F32 ? 192 : 512;
     a.part_units = partial_units(s, rows);
     a.part_o = scratch;
     a.part_ml = reinterpret_cast<float2*>(
