@@ -15,6 +15,7 @@
 // that many, and blockIdx.x is looked up in the running number of items.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "paged.hpp"
 
@@ -229,12 +230,40 @@ __device__ __forceinline__ floatx16 mma(bf16x8 a, bf16x8 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// Eight fp32 values as terms. lost: as split3x8's (bf16).
-__device__ __forceinline__ void split_terms(const float (&v)[8], bf16x8 (&t)[3], uint32_t& lost) {
-    uint4 x[3];
-    split3x8(v, x, lost);
+typedef short bf16x4 __attribute__((ext_vector_type(4)));  // bits of four bf16
+__device__ __forceinline__ floatx4 mma(bf16x4 a, bf16x4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+}
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+// (a, b) rounded to nearest bf16, a in the low half. A conversion that the
+// compiler knows: the terms go straight into MFMAs, and it keeps the wait states
+// that an MFMA needs behind a VALU write, which it does not behind inline asm.
+__device__ __forceinline__ uint32_t pair_bf16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{a, b}, bf16x2));
+}
+// N fp32 values as three terms of N bf16, each the remainder so far rounded to
+// nearest: their sum is v exactly for |v| >= 2^-109. `lost` gets bits in its low
+// half when a last term is not the whole remainder.
+template <int N, class F>
+__device__ __forceinline__ void split_terms(const float (&v)[N], F (&t)[3], uint32_t& lost) {
+#pragma clang fp contract(off)
+    typedef uint32_t words __attribute__((ext_vector_type(N / 2)));
+    words w[3];
 #pragma unroll
-    for (int i = 0; i < 3; ++i) t[i] = __builtin_bit_cast(bf16x8, x[i]);
+    for (int i = 0; i < N / 2; ++i) {
+        float a = v[2 * i], b = v[2 * i + 1];
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            w[n][i] = pair_bf16(a, b);
+            if (n == 2) break;
+            a -= from_bits(w[n][i] << 16);
+            b -= from_bits(w[n][i] & 0xffff0000u);
+            if (n == 1) lost |= bits(a) | bits(b);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < 3; ++n) t[n] = __builtin_bit_cast(F, w[n]);
 }
 __device__ __forceinline__ void split_terms(const float (&v)[8], f16x8 (&t)[2], uint32_t&) {
 #pragma clang fp contract(off)
@@ -299,15 +328,16 @@ __device__ __forceinline__ uint32_t slot_unit(const PagedArgs& p, int seq, int t
     return off < 0 ? kNoSlot : static_cast<uint32_t>(off >> 3);
 }
 
-// One wave, one column over positions lo, lo + 1 .. of every stride-th run of
-// 32 before hi, in fp32 operations on what the column sees alone: for columns
+// One wave, one column over positions lo .. lo + width - 1 of every stride
+// before hi, in fp32 operations on what the column sees alone: for columns
 // whose operands the terms do not hold, and for those beside a position that
 // is not finite and that they do not see (its zero weight would not hide it).
 // m, l: maximum (of log2 weights) and sum; o[i]: head dim lane + 64 i,
 // unnormalised.
 template <class T, int N>
 __device__ __forceinline__ void plain_column(const PagedAttnArgs& a, int seq, int row, int head,
-                                          int pq, int lo, int hi, int stride, float& m, float& l,
+                                          int pq, int lo, int hi, int width, int stride, float& m,
+                                          float& l,
                                           float (&o)[N]) {
     const PagedArgs& p = a.p;
     const int lane = threadIdx.x % kWave, D = p.head_size;
@@ -322,7 +352,7 @@ __device__ __forceinline__ void plain_column(const PagedAttnArgs& a, int seq, in
     for (int t0 = lo; t0 < hi; t0 += stride) {
         const int t = t0 + lane;
         uint32_t unit = kNoSlot;
-        if (lane < kStep && t < hi && t <= pq && !(a.window && t <= pq - a.window))
+        if (lane < width && t < hi && t <= pq && !(a.window && t <= pq - a.window))
             unit = slot_unit(p, seq, t);
         float x = -INFINITY;
         if (unit != kNoSlot) {
@@ -338,7 +368,7 @@ __device__ __forceinline__ void plain_column(const PagedAttnArgs& a, int seq, in
         l = l * alpha + wave_sum(w);
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i] *= alpha;
-        for (int i = 0; i < kStep; ++i) {
+        for (int i = 0; i < width; ++i) {
             const uint32_t u = __shfl(unit, i, kWave);
             if (u == kNoSlot) continue;
             const float wi = __shfl(w, i, kWave);
@@ -372,6 +402,8 @@ template <class T, int DP>
 struct Few {
     static constexpr int C = DP / 32, VU = DP / 16, NV = (VU + 7) / 8;
     using O = Ops<T>;
+    // Positions of a step, and of them those whose values a lane holds.
+    static constexpr int KS = O::kCacheTerms == 3 ? 16 : 32, NE = KS / 4;
     using Frag = typename O::Frag;
     static constexpr int NT = O::kTerms, KT = O::kCacheTerms;
     static constexpr int kQueryAt = kWaves * kCols * ((DP + 4) * 4 + 8);
@@ -391,12 +423,12 @@ __device__ __forceinline__ void value_terms(const Raw8<T> (&v)[8][NV], int u, F 
     x.w = __builtin_amdgcn_perm(word(v[7][n].x, wd), word(v[6][n].x, wd), sel);
     t[0] = __builtin_bit_cast(F, x);
 }
-template <class F, int NV>
-__device__ __forceinline__ void value_terms(const Raw8<float> (&v)[8][NV], int u, F (&t)[3],
+template <int NV>
+__device__ __forceinline__ void value_terms(const Raw8<float> (&v)[4][NV], int u, bf16x4 (&t)[3],
                                             uint32_t& lost) {
-    float x[8];
+    float x[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = v[e][u / 8].v[u % 8];
+    for (int e = 0; e < 4; ++e) x[e] = v[e][u / 8].v[u % 8];
     split_terms(x, t, lost);
 }
 template <class F, class T>
@@ -409,6 +441,16 @@ __device__ __forceinline__ void key_terms(const Raw8<float>& k, F (&t)[3]) {
     split_terms(k.v, t, lost);
 }
 
+// The operands of O^T += V^T P^T: as many positions a lane as a step has.
+template <class F, int NE>
+struct WeightFrag {
+    using type = F;
+};
+template <class F>
+struct WeightFrag<F, 4> {
+    using type = bf16x4;
+};
+
 // An item of the plan: columns [col0, col0 + cols) of kv head kvh of the
 // found sequence over positions [lo, hi), its partials' first unit.
 struct Item {
@@ -420,6 +462,7 @@ template <class T, int DP>
 __device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& it, char* smem) {
     using F = Few<T, DP>;
     constexpr int C = F::C, VU = F::VU, NV = F::NV, NT = F::NT, KT = F::KT;
+    constexpr int KS = F::KS, NE = F::NE, NY = KS / 16;
     constexpr int kRow = DP + 4;  // floats of a column in LDS
     // The waves' outputs; before them the query terms of fp32 caches, whose
     // keys and values take the registers (148 spilled with them): they are the
@@ -491,16 +534,18 @@ __device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& 
 
     const T* kc = static_cast<const T*>(a.kc) + kvh * p.head_stride;
     const T* vc = static_cast<const T*>(a.vc) + kvh * p.head_stride;
-    // Lane l holds position l % 32 of a step. Positions that are not there
+    // Lane l holds position l % KS of a step. Positions that are not there
     // read slot 0 and count for nothing.
     auto units = [&](int t0) {
-        const int t = t0 + (lane & 31);
+        const int t = t0 + (lane & (KS - 1));
         return t < hi ? slot_unit(p, f.seq, t) : kNoSlot;
     };
-    Raw8<T> k[2][C], v[8][NV];
+    auto place = [&](int e) { return 4 * g + (e < 4 ? e : 12 + e); };  // of a lane's e-th position
+    using Values = Raw8<T>[NE][NV];
+    Raw8<T> k[NY][C];
     auto load_k = [&](uint32_t u) {
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
+        for (int y = 0; y < NY; ++y) {
             const uint32_t x = __shfl(u, 16 * y + j, kWave);
             const T* src = kc + static_cast<std::size_t>(x == kNoSlot ? 0 : x) * 8;
 #pragma unroll
@@ -510,10 +555,10 @@ __device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& 
             }
         }
     };
-    auto load_v = [&](uint32_t u) {
+    auto load_v = [&](uint32_t u, Values& v) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t x = __shfl(u, 4 * g + (e < 4 ? e : 12 + e), kWave);
+        for (int e = 0; e < NE; ++e) {
+            const uint32_t x = __shfl(u, place(e), kWave);
             const T* src = vc + static_cast<std::size_t>(x == kNoSlot ? 0 : x) * 8;
 #pragma unroll
             for (int n = 0; n < NV; ++n) {
@@ -541,91 +586,103 @@ __device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& 
 #pragma unroll
     for (int u = 0; u < VU; ++u) o[u] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-    constexpr int kStride = kStep * kWaves;
-    int t0 = lo + w * kStep;
-    if (t0 < hi) {
-        uint32_t u = units(t0);
-        load_k(u);
-        load_v(u);
-        while (true) {
-            const uint32_t un = units(t0 + kStride);
-            floatx4 s[2];
+    constexpr int kStride = KS * kWaves;
+    int t0 = lo + w * KS;
+    uint32_t u = kNoSlot;
+    // One step with its values in v; the next one's keys are loaded after the
+    // scores, its values into vn before them or, where vn is v, after their
+    // products. False: it was the last.
+    auto step = [&](Values& v, Values& vn, auto ahead) {
+        const uint32_t un = units(t0 + kStride);
+        const bool more = t0 + kStride < hi;
+        if (ahead && more) load_v(un, vn);
+        floatx4 s[NY];
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                s[y] = floatx4{0.f, 0.f, 0.f, 0.f};
+        for (int y = 0; y < NY; ++y) {
+            s[y] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    typename F::Frag kt[KT];
-                    key_terms(k[y][c], kt);
-                    if constexpr (kQueryLds) {
-                        typename F::Frag qt[NT];
+            for (int c = 0; c < C; ++c) {
+                typename F::Frag kt[KT];
+                key_terms(k[y][c], kt);
+                if constexpr (kQueryLds) {
+                    typename F::Frag qt[NT];
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) qt[t] = q_s[(c * NT + t) * kWave + lane];
-                        mma_terms(kt, qt, s[y]);
-                        // One split's terms at a time, not all of them in registers.
-                        if constexpr (KT == 3) __builtin_amdgcn_sched_barrier(0);
-                    } else {
-                        mma_terms(kt, q[c], s[y]);
+                    for (int t = 0; t < NT; ++t) qt[t] = q_s[(c * NT + t) * kWave + lane];
+                    mma_terms(kt, qt, s[y]);
+                } else {
+                    mma_terms(kt, q[c], s[y]);
+                }
+            }
+        }
+        if (more) load_k(un);
+        float x[NE];
+#pragma unroll
+        for (int e = 0; e < NE; ++e) x[e] = NT == 2 ? s[e / 4][e % 4] * unscale : s[e / 4][e % 4];
+        // Positions that are there, of the step's.
+        constexpr uint32_t kAll = KS == 32 ? 0xffffffffu : (1u << (KS & 31)) - 1;
+        const uint32_t there = static_cast<uint32_t>(__ballot(u != kNoSlot)) & kAll;
+        if (there != kAll || t0 < all_lo || t0 + KS - 1 > all_hi) {
+#pragma unroll
+            for (int e = 0; e < NE; ++e) {
+                const int r = place(e), t = t0 + r;
+                const bool seen = (there >> r & 1) && t <= pq && !(a.window && t <= pq - a.window);
+                x[e] = seen ? x[e] : -INFINITY;
+            }
+            if (there != kAll) {
+#pragma unroll
+                for (int e = 0; e < NE; ++e)
+                    if (!(there >> place(e) & 1)) {
+#pragma unroll
+                        for (int n = 0; n < NV; ++n) v[e][n].zero();
                     }
-                }
             }
-            const bool more = t0 + kStride < hi;
-            if (more) load_k(un);
-            float x[8];
+        }
+        float mb = x[0];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = NT == 2 ? s[e / 4][e % 4] * unscale : s[e / 4][e % 4];
-            // Positions that are there, of the step's 32.
-            const uint32_t there = static_cast<uint32_t>(__ballot(u != kNoSlot));
-            if (there != 0xffffffffu || t0 < all_lo || t0 + kStep - 1 > all_hi) {
+        for (int e = 1; e < NE; ++e) mb = fmaxf(mb, x[e]);
+        const float mn = fmaxf(m, max32(max16(mb)));
+        if (__ballot(mn > m)) {
+            const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            l *= alpha;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int r = 4 * g + (e < 4 ? e : 12 + e), t = t0 + r;
-                    const bool seen =
-                        (there >> r & 1) && t <= pq && !(a.window && t <= pq - a.window);
-                    x[e] = seen ? x[e] : -INFINITY;
-                }
-                if (there != 0xffffffffu) {
+            for (int y = 0; y < VU; ++y) o[y] *= alpha;
+            m = mn;
+        }
+        const float base = mn == -INFINITY ? 0.0f : mn;
+        float pw[NE];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (!(there >> (4 * g + (e < 4 ? e : 12 + e)) & 1)) {
+        for (int e = 0; e < NE; ++e) {
+            pw[e] = __builtin_amdgcn_exp2f(x[e] - base);
+            l += pw[e];
+            pw[e] *= F::O::kWeight;
+        }
+        typename WeightFrag<typename F::Frag, NE>::type pt[NT];
+        uint32_t lost_p = 0;
+        split_terms(pw, pt, lost_p);
 #pragma unroll
-                            for (int n = 0; n < NV; ++n) v[e][n].zero();
-                        }
-                }
+        for (int y = 0; y < VU; ++y) {
+            typename WeightFrag<typename F::Frag, NE>::type vt[KT];
+            value_terms(v, y, vt, lost_v);
+            mma_terms(vt, pt, o[y]);
+        }
+        if (!more) return false;
+        if (!ahead) load_v(un, vn);
+        u = un;
+        t0 += kStride;
+        return true;
+    };
+    if (t0 < hi) {
+        Raw8<T> v[NE][NV];
+        u = units(t0);
+        load_k(u);
+        load_v(u, v);
+        if constexpr (KT == 3) {
+            Raw8<T> v2[NE][NV];
+            while (step(v, v2, std::true_type{}) && step(v2, v, std::true_type{})) {
             }
-            float mb = x[0];
-#pragma unroll
-            for (int e = 1; e < 8; ++e) mb = fmaxf(mb, x[e]);
-            const float mn = fmaxf(m, max32(max16(mb)));
-            if (__ballot(mn > m)) {
-                const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-                l *= alpha;
-#pragma unroll
-                for (int y = 0; y < VU; ++y) o[y] *= alpha;
-                m = mn;
+        } else {
+            while (step(v, v, std::false_type{})) {
             }
-            const float base = mn == -INFINITY ? 0.0f : mn;
-            float pw[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                pw[e] = __builtin_amdgcn_exp2f(x[e] - base);
-                l += pw[e];
-                pw[e] *= F::O::kWeight;
-            }
-            typename F::Frag pt[NT];
-            uint32_t lost_p = 0;
-            split_terms(pw, pt, lost_p);
-#pragma unroll
-            for (int y = 0; y < VU; ++y) {
-                typename F::Frag vt[KT];
-                value_terms(v, y, vt, lost_v);
-                mma_terms(vt, pt, o[y]);
-                if constexpr (KT == 3) __builtin_amdgcn_sched_barrier(0);
-            }
-            if (!more) break;
-            load_v(un);
-            u = un;
-            t0 += kStride;
         }
     }
     l = sum32(sum16(l));
@@ -658,7 +715,7 @@ __device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& 
         redo &= redo - 1;
         float po[DP / kWave], pm, pl;
         plain_column<T, DP / kWave>(a, f.seq, __shfl(row, c, kWave), __shfl(head, c, kWave),
-                                    __shfl(pq, c, kWave), lo + w * kStep, hi, kStride, pm, pl, po);
+                                    __shfl(pq, c, kWave), lo + w * KS, hi, KS, kStride, pm, pl, po);
 #pragma unroll
         for (int n = 0; n < DP / kWave; ++n) o_s[w][c][lane + kWave * n] = po[n];
         if (lane == 0) ml_s[w][c] = make_float2(pm, pl);
@@ -1013,7 +1070,8 @@ __device__ __forceinline__ void wide_item(const PagedAttnArgs& a, const Item& it
         if (wc + c >= it.cols) break;
         float po[DP / kWave], pm, pl;
         const int prow = __shfl(row, c, kWave), phead = __shfl(head, c, kWave);
-        plain_column<T, DP / kWave>(a, f.seq, prow, phead, __shfl(pq, c, kWave), lo, hi, kStep, pm, pl, po);
+        plain_column<T, DP / kWave>(a, f.seq, prow, phead, __shfl(pq, c, kWave), lo, hi, kStep,
+                                    kStep, pm, pl, po);
         const std::size_t ppc = static_cast<std::size_t>(it.unit) * kCols + wc + c;
         float* pdst = f.runs > 1 ? a.part_o + ppc * D : a.out + prow * a.out_stride + phead * D;
         const float pby = f.runs > 1 ? 1.0f : pl == 0.0f ? 0.0f : 1.0f / pl;
