@@ -439,6 +439,15 @@ int em_model_destroy(em_model* m);
  * safe from several host threads at once. */
 int em_model_forward(em_model* m, const int* tokens, size_t n, size_t pos, float* logits);
 
+/* em_model_forward with the next token drawn from its logits on the GPU, as
+ * em_sample draws it from the number u: the logits are not copied to the host.
+ * *token gets it, *logprob (unless NULL) its log-probability; both are written
+ * when the call succeeds. The settings' neutral values are 1, 0, 1 and 0. A
+ * one-token call is captured as em_model_forward's is, once each for calls
+ * without and with a top_k above 0. EM_EINVAL for a vocabulary past 2^20. */
+int em_model_sample(em_model* m, const int* tokens, size_t n, size_t pos, float temperature,
+                    int top_k, float top_p, float min_p, float u, int* token, float* logprob);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,7 +35,7 @@ EXPORTS = (
     "em_attention_check", "em_attention_scratch_floats", "em_attention",
     "em_paged_check", "em_paged_append", "em_paged_attention_scratch_floats",
     "em_paged_attention", "em_sample_scratch_bytes", "em_sample",
-    "em_model_create", "em_model_destroy", "em_model_forward",
+    "em_model_create", "em_model_destroy", "em_model_forward", "em_model_sample",
     "em_model_load", "em_model_config_get", "em_model_read_weight",
 )
 CACHE_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
@@ -180,6 +180,8 @@ def lib() -> ctypes.CDLL:
                                       ctypes.POINTER(_vp)]
         L.em_model_destroy.argtypes = [_vp]
         L.em_model_forward.argtypes = [_vp, _vp, _sz, _sz, _vp]
+        fl = ctypes.c_float
+        L.em_model_sample.argtypes = [_vp, _vp, _sz, _sz, fl, ctypes.c_int, fl, fl, fl, _vp, _vp]
         L.em_model_load.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(_vp)]
         L.em_model_config_get.argtypes = [_vp, ctypes.POINTER(ModelConfig)]
         L.em_model_read_weight.argtypes = [_vp, ctypes.c_char_p, _sz, _vp, _sz]
@@ -713,6 +715,18 @@ class Model:
         out = np.empty((int(self.config["vocab_size"]),), np.float32)
         _check(lib().em_model_forward(self.h, t.ctypes.data, t.size, pos, out.ctypes.data))
         return out
+
+    def sample(self, tokens, pos: int, u: float, temperature: float = 1.0, top_k: int = 0,
+               top_p: float = 1.0, min_p: float = 0.0):
+        """em_model_sample: (token, log-probability) drawn by u from the logits
+        that forward(tokens, pos) returns."""
+        import numpy as np
+        t = np.ascontiguousarray(np.atleast_1d(tokens), np.int32)
+        token, logprob = ctypes.c_int(), ctypes.c_float()
+        _check(lib().em_model_sample(self.h, t.ctypes.data, t.size, pos, temperature, top_k,
+                                     top_p, min_p, u, ctypes.addressof(token),
+                                     ctypes.addressof(logprob)))
+        return token.value, logprob.value
 
     def close(self) -> None:
         if getattr(self, "h", None):

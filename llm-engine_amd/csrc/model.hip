@@ -33,6 +33,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <memory>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -118,6 +119,20 @@ __global__ __launch_bounds__(kThreads) void rope_cache_kernel(Summed src, int qk
         value_cache[static_cast<std::size_t>(pos) * kv_dim + t] =
             summed(src, i, dim + kv_dim + t);
     }
+}
+
+// One row's sampling settings, as the host writes them.
+struct DrawSettings {
+    float temperature, top_p, min_p, u;
+    int top_k;
+};
+// The host's pinned settings into device memory, word by word with
+// system-scope loads, as embed_kernel reads the feed: a replayed step then
+// draws by what the host wrote for it.
+__global__ void draw_settings_kernel(const int* __restrict__ host, int* __restrict__ device) {
+    const int i = threadIdx.x;
+    if (i < static_cast<int>(sizeof(DrawSettings) / sizeof(int)))
+        device[i] = __hip_atomic_load(host + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
 // hb[r][c] = silu(g) * u with g = gu[r][c], u = gu[r][hidden + c]
@@ -268,8 +283,20 @@ public:
 
     // Returns EM_OK or an error code (message recorded with fail()).
     int run(const int* tokens, std::size_t n, std::size_t pos, float* logits);
+    // The same, but the next token is drawn from the logits on the GPU.
+    int sample(const int* tokens, std::size_t n, std::size_t pos, const DrawSettings& draw,
+               int* token, float* logprob);
 
 private:
+    // One-token steps as captured, replayed while no buffer has moved.
+    struct Step {
+        GraphExec graph;
+        std::size_t generation = 0;
+    };
+    int feed(const int* tokens, std::size_t n, std::size_t pos, Step& step, bool draw, bool top_k,
+             bool& eager_step);
+    void capture(Step& step, bool draw, bool top_k);
+    void enqueue_step(int n, bool draw, bool top_k);
     void init_runtime();
     void quantize_proj(Proj& p);
     void upload(Buf<float>& b, const float* src, std::size_t count);
@@ -286,7 +313,7 @@ private:
     bool qkv_exact_split(int n, LayerDev& L, bool* roped);
     bool swiglu_w2(const Summed& gu, const Proj& w2, bool* wrote_ssq);
     void reserve_rows(std::size_t n);
-    void enqueue(int n);
+    void enqueue(int n, float* logits);
     std::size_t buffers_generation() const { return own_generation_ + scratch_generation(); }
 
     // Declared first, destroyed last: the buffers below are freed after the
@@ -336,8 +363,16 @@ private:
     Pinned<int> feed_host_;  // [pos, tokens...]
     Buf<int> feed_dev_;
     Pinned<float> logits_host_;
-    GraphExec graph_;
-    std::size_t graph_generation_ = 0;
+    Step forward_;
+    // sample(): logits that stay on the GPU, the settings there and as the host
+    // writes them, the token and its log-probability (allocated by its first
+    // call), and a step each without and with a top-k.
+    Buf<float> logits_dev_;
+    Buf<DrawSettings> draw_dev_;
+    Buf<char> draw_scratch_;
+    std::unique_ptr<Pinned<DrawSettings>> draw_host_;
+    std::unique_ptr<Pinned<float>> drawn_;
+    Step drawing_[2];
 };
 
 Model::Model(const em_model_config& c, const float* emb, const em_layer_weights* layers,
@@ -907,7 +942,7 @@ void Model::reserve_rows(std::size_t n) {
     ++own_generation_;
 }
 
-void Model::enqueue(int n) {
+void Model::enqueue(int n, float* logits) {
     const int D = static_cast<int>(cfg_.dim), H = static_cast<int>(cfg_.hidden_dim);
     const int KV = static_cast<int>(shape_.kv_stride), hs = shape_.head_size;
     const int qkv_cols = static_cast<int>(shape_.q_stride);
@@ -995,24 +1030,45 @@ void Model::enqueue(int n) {
             have_ssq = false;
         }
     }
-    // Only the last row's logits are returned, written by the classifier's
-    // kernel straight into the host's pinned buffer.
+    // Only the last row's logits are returned: forward() has the classifier's
+    // kernel write them straight into the host's pinned buffer.
     const float* x_last = x_.p + static_cast<std::size_t>(n - 1) * D;
     if (have_ssq) {
         const MatmulArgs a =
-            gemv_args(1, x_last, wcls_, logits_host_.dev, rms_final_.p, false, ssq_.p);
+            gemv_args(1, x_last, wcls_, logits, rms_final_.p, false, ssq_.p);
         if (q8_) {
             run_skinny<int8_t>(a);
         } else {
             run_skinny<float>(a);
         }
     } else {
-        project(1, x_last, wcls_, logits_host_.dev, rms_final_.p, false);
+        project(1, x_last, wcls_, logits, rms_final_.p, false);
     }
     check(hipGetLastError(), "launch");
 }
 
-int Model::run(const int* tokens, std::size_t n, std::size_t pos, float* logits) {
+// The forward pass of n tokens to the host's logits, or to the GPU's and a token
+// drawn from them.
+void Model::enqueue_step(int n, bool draw, bool top_k) {
+    if (!draw) {
+        enqueue(n, logits_host_.dev);
+        return;
+    }
+    hipLaunchKernelGGL(draw_settings_kernel, dim3(1), dim3(kWave), 0, stream_,
+                       reinterpret_cast<const int*>(draw_host_->dev),
+                       reinterpret_cast<int*>(draw_dev_.p));
+    enqueue(n, logits_dev_.p);
+    const DrawSettings* d = draw_dev_.p;
+    const em_sampling set{&d->temperature, top_k ? &d->top_k : nullptr, &d->top_p, &d->min_p};
+    if (em_sample(1, cfg_.vocab_size, logits_dev_.p, cfg_.vocab_size, &d->u, &set,
+                  reinterpret_cast<int*>(drawn_->dev), drawn_->dev + 1, draw_scratch_.p,
+                  stream_) != EM_OK)
+        throw DeviceError(em_last_error());
+}
+
+// Feeds and waits. eager_step: a one-token step ran without its graph.
+int Model::feed(const int* tokens, std::size_t n, std::size_t pos, Step& step, bool draw,
+                bool top_k, bool& eager_step) {
     // check_feed, model.cpp:165-177: the CPU model's exact rules and messages.
     for (std::size_t i = 0; i < n; ++i) {
         if (tokens[i] < 0 || static_cast<std::size_t>(tokens[i]) >= cfg_.vocab_size)
@@ -1027,37 +1083,64 @@ int Model::run(const int* tokens, std::size_t n, std::size_t pos, float* logits)
     feed_host_.p[0] = static_cast<int>(pos);
     std::memcpy(feed_host_.p + 1, tokens, n * sizeof(int));
 
-    const bool replay = n == 1 && graph_.g && graph_generation_ == buffers_generation();
+    const bool replay = n == 1 && step.graph.g && step.generation == buffers_generation();
     if (replay) {
-        check(hipGraphLaunch(graph_.g, stream_), "graph launch");
+        check(hipGraphLaunch(step.graph.g, stream_), "graph launch");
     } else {
-        enqueue(static_cast<int>(n));
+        enqueue_step(static_cast<int>(n), draw, top_k);
     }
     check(hipStreamSynchronize(stream_), "forward");
     filled_ = pos + n;
-    std::memcpy(logits, logits_host_.p, cfg_.vocab_size * sizeof(float));
+    eager_step = n == 1 && !replay;
+    return EM_OK;
+}
 
-    // After an eager one-token run every buffer the step needs has grown, so
-    // capturing allocates nothing.
-    if (n == 1 && !replay) {
-        graph_.reset();
-        hipGraph_t graph = nullptr;
-        check(hipStreamBeginCapture(stream_, hipStreamCaptureModeThreadLocal), "begin capture");
-        try {
-            enqueue(1);
-        } catch (...) {
-            (void)hipStreamEndCapture(stream_, &graph);
-            if (graph) (void)hipGraphDestroy(graph);
-            throw;
-        }
-        check(hipStreamEndCapture(stream_, &graph), "end capture");
-        hipGraphExec_t exec = nullptr;
-        const hipError_t err = hipGraphInstantiate(&exec, graph, nullptr, nullptr, 0);
-        (void)hipGraphDestroy(graph);
-        check(err, "instantiate graph");
-        graph_.g = exec;
-        graph_generation_ = buffers_generation();
+// After an eager one-token step every buffer it needs has grown, so capturing
+// it allocates nothing.
+void Model::capture(Step& step, bool draw, bool top_k) {
+    step.graph.reset();
+    hipGraph_t graph = nullptr;
+    check(hipStreamBeginCapture(stream_, hipStreamCaptureModeThreadLocal), "begin capture");
+    try {
+        enqueue_step(1, draw, top_k);
+    } catch (...) {
+        (void)hipStreamEndCapture(stream_, &graph);
+        if (graph) (void)hipGraphDestroy(graph);
+        throw;
     }
+    check(hipStreamEndCapture(stream_, &graph), "end capture");
+    hipGraphExec_t exec = nullptr;
+    const hipError_t err = hipGraphInstantiate(&exec, graph, nullptr, nullptr, 0);
+    (void)hipGraphDestroy(graph);
+    check(err, "instantiate graph");
+    step.graph.g = exec;
+    step.generation = buffers_generation();
+}
+
+int Model::run(const int* tokens, std::size_t n, std::size_t pos, float* logits) {
+    bool eager_step = false;
+    if (const int rc = feed(tokens, n, pos, forward_, false, false, eager_step)) return rc;
+    std::memcpy(logits, logits_host_.p, cfg_.vocab_size * sizeof(float));
+    if (eager_step) capture(forward_, false, false);
+    return EM_OK;
+}
+
+int Model::sample(const int* tokens, std::size_t n, std::size_t pos, const DrawSettings& draw,
+                  int* token, float* logprob) {
+    if (!drawn_) {
+        logits_dev_.alloc(cfg_.vocab_size);
+        draw_dev_.alloc(1);
+        draw_scratch_.alloc(std::max<std::size_t>(1, em_sample_scratch_bytes(1, cfg_.vocab_size)));
+        draw_host_ = std::make_unique<Pinned<DrawSettings>>(1);
+        drawn_ = std::make_unique<Pinned<float>>(2);
+    }
+    *draw_host_->p = draw;
+    const bool top_k = draw.top_k > 0;
+    bool eager_step = false;
+    if (const int rc = feed(tokens, n, pos, drawing_[top_k], true, top_k, eager_step)) return rc;
+    std::memcpy(token, drawn_->p, sizeof(int));
+    if (logprob) *logprob = drawn_->p[1];
+    if (eager_step) capture(drawing_[top_k], true, top_k);
     return EM_OK;
 }
 
@@ -1182,6 +1265,21 @@ int em_model_forward(em_model* m, const int* tokens, size_t n, size_t pos, float
     if (!tokens || !logits) return fail(EM_EINVAL, "forward: null pointer");
     try {
         return m->impl.run(tokens, n, pos, logits);
+    } catch (const std::exception& e) {
+        return fail(EM_EDEVICE, e.what());
+    }
+}
+
+int em_model_sample(em_model* m, const int* tokens, size_t n, size_t pos, float temperature,
+                    int top_k, float top_p, float min_p, float u, int* token, float* logprob) {
+    if (!m) return fail(EM_EINVAL, "model_sample: null model");
+    if (n == 0) return fail(EM_EINVAL, "model_sample: no tokens");
+    if (!tokens || !token) return fail(EM_EINVAL, "model_sample: null pointer");
+    if (m->impl.config().vocab_size > (size_t{1} << 20))
+        return fail(EM_EINVAL, "model_sample: a vocabulary of more than 2^20");
+    try {
+        return m->impl.sample(tokens, n, pos, em::DrawSettings{temperature, top_p, min_p, u, top_k},
+                              token, logprob);
     } catch (const std::exception& e) {
         return fail(EM_EDEVICE, e.what());
     }

@@ -47,6 +47,7 @@ struct PagedAttnArgs {
     int wide;       // sequences may take wide items
     int slots;      // workgroups to spread the positions over
     int min_wide;   // positions of a wide item at least
+    float wide_cost;  // what a position costs a wide item, in a narrow one's
     float* part_o;  // [unit][16 columns][head_size], a unit an item's 16 columns
     float2* part_ml;
     int part_units;
@@ -96,7 +97,7 @@ __device__ __forceinline__ int wave_scan_int(int v) {  // inclusive
     return v;
 }
 
-// All columns' positions over the slots. Narrow items take half of that where a
+// What all columns' positions cost over the slots. Narrow items take half of that where a
 // sequence would be only a few of them: rounding leaves items of up to one and
 // a half lengths, which twice as many even out (64 sequences of 500 to 4000
 // positions 167 / 146 us, 2 of 100000 189 / 195; a cut costs a wide item its
@@ -112,7 +113,7 @@ __device__ __forceinline__ RunLength run_length(const PagedAttnArgs& a) {
         if (s0 + lane < a.p.n_seqs) {
             const SeqWork w = seq_work(a, s0 + lane);
             n = static_cast<float>(w.tiles);
-            t = n * static_cast<float>(w.span);
+            t = n * static_cast<float>(w.span) * (w.width == kWideCols ? a.wide_cost : 1.0f);
         }
         total += wave_sum(t);
         tiles += wave_sum(n);
@@ -120,7 +121,8 @@ __device__ __forceinline__ RunLength run_length(const PagedAttnArgs& a) {
     const float kv = static_cast<float>(a.p.n_kv_heads), slots = static_cast<float>(a.slots);
     const float run = total * kv / slots;
     const float part = tiles * kv * 16.0f > slots ? 0.5f : 1.0f;
-    return {fmaxf(run * part, static_cast<float>(kMinRun)), fmaxf(run, static_cast<float>(a.min_wide))};
+    return {fmaxf(run * part, static_cast<float>(kMinRun)),
+            fmaxf(run / a.wide_cost, static_cast<float>(a.min_wide))};
 }
 
 // Runs of a sequence: its positions over a run's length, to the nearest whole
@@ -781,6 +783,7 @@ struct Wide {
     static constexpr bool kQueryLds = NT == 3 && DP <= 128;
     static constexpr int kQueryAt = kBufs * kStage;
     static constexpr int kLds = kQueryAt + (kQueryLds ? kWaves * C * kWave * 16 : 0);
+    static_assert(kWaves * 32 * (8 * DU + 4) * 4 <= kLds);
     static constexpr int kLoads = kStep * (DP / 8) / kThreads;  // units a thread, of K and of V
 };
 
@@ -1022,7 +1025,8 @@ __device__ __forceinline__ void wide_item(const PagedAttnArgs& a, const Item& it
             if (more) store(mask(units), smem + (W::kBufs == 2 ? ((s + 1) & 1) * W::kStage : 0));
         }
     }
-    // Whether any wave stored a value that dropped bits.
+    // Every wave is through with the stages in LDS. v_lost: whether any stored a
+    // value that dropped bits.
     bool v_lost = false;
     if constexpr (KT == 3) {
         auto* flag = reinterpret_cast<int*>(smem);
@@ -1033,6 +1037,7 @@ __device__ __forceinline__ void wide_item(const PagedAttnArgs& a, const Item& it
         __syncthreads();
         v_lost = *flag != 0;
     }
+    __syncthreads();
     if (idle) return;
     l = sum32(l);
     float low = INFINITY;
@@ -1049,21 +1054,38 @@ __device__ __forceinline__ void wide_item(const PagedAttnArgs& a, const Item& it
     bad |= !(l < INFINITY);
     unsigned long long redo = __ballot(bad);
     redo = (redo | redo >> 32) & 0xffffffffull;
-    const bool mine = wc + j < it.cols;
-    const std::size_t pc = static_cast<std::size_t>(it.unit) * kCols + cin;
-    float* dst = f.runs > 1 ? a.part_o + pc * D : a.out + row * a.out_stride + head * D;
+    // Head dims DU 8 y .. DU 8 (y + 1) of the wave's columns at a time through
+    // LDS, so that a column's are written in whole lines (64 lanes' eight bytes of
+    // as many rows: 15 us for 128 columns of 128 in every workgroup at once).
+    constexpr int CH = 8 * DU, kChRow = CH + 4, kLanes = CH / 4;
     const float by = (f.runs > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l) * (1.0f / W::O::kWeight);
-    if (mine && !(redo >> j & 1)) {
+    float* o_s = reinterpret_cast<float*>(smem) + w * 32 * kChRow;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int d = DU * (8 * (r / 4) + 4 * h + r % 4);
+    for (int y = 0; y < 4; ++y) {
 #pragma unroll
-            for (int u = 0; u < DU; u += 2)
-                if (d + u < D)
-                    *reinterpret_cast<float2*>(dst + d + u) = make_float2(o[u][r] * by, o[u + 1][r] * by);
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int u = 0; u < DU; ++u) o_s[j * kChRow + DU * (4 * h + r) + u] = o[u][4 * y + r] * by;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int x = 0; x < 32; x += kWave / kLanes) {
+            const int c = x + lane / kLanes, at = lane % kLanes * 4, d = CH * y + at;
+            const floatx4 z = *reinterpret_cast<const floatx4*>(o_s + c * kChRow + at);
+            if (wc + c < it.cols && !(redo >> c & 1) && d < D) {
+                const int cc = it.col0 + wc + c;
+                float* dst = f.runs > 1
+                                 ? a.part_o + (static_cast<std::size_t>(it.unit) * kCols + wc + c) * D
+                                 : a.out + (f.w.row0 + cc / p.group) * a.out_stride +
+                                       (kvh * p.group + cc % p.group) * D;
+                *reinterpret_cast<floatx4*>(dst + d) = z;
+            }
         }
-        if (f.runs > 1 && h == 0) a.part_ml[pc] = make_float2(m, l);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
+    if (f.runs > 1 && h == 0 && wc + j < it.cols && !(redo >> j & 1))
+        a.part_ml[static_cast<std::size_t>(it.unit) * kCols + cin] = make_float2(m, l);
     while (redo) {
         const int c = __ffsll(redo) - 1;
         redo &= redo - 1;
@@ -1277,6 +1299,10 @@ void run_paged_attention(PagedAttnArgs a, const em_paged_shape& s, float* scratc
     // one of 1205 rows of 24 heads of 96 85 / 116; eight of up to 466 rows of 20
     // heads of 80 (fp16) 50 / 34.
     a.min_wide = s.type == EM_CACHE_F32 ? 192 : 512;
+    // With two workgroups on a CU a wide item takes 175 ns a position of heads of
+    // 128 (fp32; bf16 96, fp16 75), a narrow one that reads at HBM's rate 50 (fp32
+    // 100, of which the cache holds some).
+    a.wide_cost = s.type == EM_CACHE_F32 ? 3.0f : s.type == EM_CACHE_BF16 ? 2.0f : 1.5f;
     a.part_units = partial_units(s, rows);
     a.part_o = scratch;
     a.part_ml = reinterpret_cast<float2*>(

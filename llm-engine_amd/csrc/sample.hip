@@ -32,7 +32,8 @@ constexpr int kSampleThreads = 1024;
 constexpr int kSampleWaves = kSampleThreads / kWave;
 constexpr int kChunk = 4 * kWave;  // logits a wave reads at once
 constexpr int kMaxVocab = 1 << 20;
-constexpr int kBins = 2048;
+// Bins of a histogram: what LDS holds beside a row, and more where it need not.
+constexpr int kHeldBins = 2048, kWideBins = 4096;
 constexpr int kList = 512;   // tokens of a bin that are ranked against each other
 constexpr int kShort = 128;  // a list that holds all that may be kept
 
@@ -133,24 +134,63 @@ __device__ __forceinline__ u64 share_up(u64 total, float share) {
     return __umul64hi(total, f) + (total * f != 0);
 }
 
-template <class T>
-__device__ __forceinline__ T wave_scan(T v) {  // inclusive
-    const int lane = threadIdx.x % kWave;
+// v of the lane that a DPP control names, `none` where there is none or the row
+// is masked out: a register move, where a shuffle goes through LDS.
+template <int CTRL, int ROWS, class T>
+__device__ __forceinline__ T dpp_move(T v, T none) {
+    static_assert(sizeof(T) == 4 || sizeof(T) == 8);
+    int o[sizeof(T) / 4], x[sizeof(T) / 4];
+    __builtin_memcpy(o, &none, sizeof(T));
+    __builtin_memcpy(x, &v, sizeof(T));
 #pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        const T o = __shfl_up(v, d, kWave);
-        if (lane >= d) v += o;
-    }
+    for (unsigned i = 0; i < sizeof(T) / 4; ++i)
+        x[i] = __builtin_amdgcn_update_dpp(o[i], x[i], CTRL, ROWS, 0xf, false);
+    __builtin_memcpy(&v, x, sizeof(T));
     return v;
 }
+// Inclusive scan over a wave's lanes: within rows of 16 by shifts of 1, 2, 4
+// and 8, then each odd row takes the last of the row before, then the upper two
+// that of the lower two.
+template <class T, class Op>
+__device__ __forceinline__ T wave_scan(T v, T none, Op op) {
+    v = op(v, dpp_move<0x111, 0xf>(v, none));
+    v = op(v, dpp_move<0x112, 0xf>(v, none));
+    v = op(v, dpp_move<0x114, 0xf>(v, none));
+    v = op(v, dpp_move<0x118, 0xf>(v, none));
+    v = op(v, dpp_move<0x142, 0xa>(v, none));
+    v = op(v, dpp_move<0x143, 0xc>(v, none));
+    return v;
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+    return wave_scan(v, T(0), [](T a, T b) { return a + b; });
+}
+// The last lane's value, in every lane.
+template <class T>
+__device__ __forceinline__ T last_lane(T v) {
+    int x[sizeof(T) / 4];
+    __builtin_memcpy(x, &v, sizeof(T));
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(T) / 4; ++i) x[i] = __builtin_amdgcn_readlane(x[i], kWave - 1);
+    __builtin_memcpy(&v, x, sizeof(T));
+    return v;
+}
+__device__ __forceinline__ float wave_top(float v) {
+    return last_lane(wave_scan(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); }));
+}
+__device__ __forceinline__ int wave_least(int v) {
+    return last_lane(wave_scan(v, 0x7fffffff, [](int a, int b) { return min(a, b); }));
+}
 
+template <int BINS>
 struct SampleShared {
-    u64 weight[kBins];  // the bins'; once they have been read, the list's
-    uint32_t count[kBins];
+    static constexpr int kBins = BINS;
+    u64 weight[BINS];  // the bins'; once they have been read, the list's
+    uint32_t count[BINS];
     uint32_t list[kList];
     int list_at[kList];
     double roots[2 * kRoots];
-    double part[kSampleWaves];
+    double part[kSampleWaves], sums[32];
     u64 part64[kSampleWaves];
     float part_hi[kSampleWaves], part_lo[kSampleWaves];
     uint32_t part_n[kSampleWaves];
@@ -161,7 +201,7 @@ struct SampleShared {
 
 // Chunks a wave whose row LDS (160 KB) holds beside SampleShared.
 constexpr int kHeldChunks = 8;
-static_assert(sizeof(SampleShared) + kHeldChunks * kSampleWaves * kChunk * sizeof(float) <= 160 * 1024);
+static_assert(sizeof(SampleShared<kHeldBins>) + kHeldChunks * kSampleWaves * kChunk * sizeof(float) <= 160 * 1024);
 
 template <class T>
 __device__ __forceinline__ T shfl(T v, int lane) { return __shfl(v, lane, kWave); }
@@ -261,11 +301,222 @@ struct Row {
     }
 };
 
-template <bool HELD>
-__global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a) {
-    __shared__ SampleShared s;
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-    extern __shared__ __attribute__((aligned(16))) float held[];
+// A row's settings; `top_k` 0: off.
+struct Settings {
+    float temperature, top_p;
+    bool greedy;
+    int top_k;
+    double min_p, draw;
+    __device__ __forceinline__ Settings(const SampleArgs& a, int r) {
+        temperature = a.temperature ? a.temperature[r] : 1.0f;
+        greedy = !(temperature > 0.0f);
+        top_k = a.top_k && a.top_k[r] < a.vocab ? max(0, a.top_k[r]) : 0;
+        top_p = a.top_p ? a.top_p[r] : 1.0f;
+        const float mp = a.min_p ? a.min_p[r] : 0.0f, u = a.u[r];
+        min_p = mp > 0.0f ? fmin(static_cast<double>(mp), 1.0) : 0.0;
+        draw = u > 0.0f ? fmin(static_cast<double>(u), 1.0) : 0.0;
+    }
+};
+
+__device__ __forceinline__ Weigh weigh_of(const SampleArgs& a, const Settings& set, float top,
+                                          const double* roots) {
+    const float T = set.temperature;
+    return {top, top == INFINITY, fmaxf(static_cast<float>(top - 60.0 * T), -3.4028235e38f),
+            set.greedy ? 0.0 : kRoots * 1.4426950408889634074 / T, a.bits, roots};
+}
+// No logit below this weighs min_p (a thousandth of T and the fp32 roundings
+// of the sum are left for the comparison in 64 bits), or anything.
+__device__ __forceinline__ float cut_of(const Settings& set, const Weigh& weigh) {
+    if (weigh.endless || set.min_p == 0.0) return weigh.least;
+    return fmaxf(weigh.least, static_cast<float>(weigh.top + (log(set.min_p) - 1e-3) * set.temperature -
+                                                 1e-6 * fabs(static_cast<double>(weigh.top))));
+}
+// The histogram's bin of x; inv: bins over the range they cover.
+template <int BINS>
+__device__ __forceinline__ int bin_at(float x, float top, float inv) {
+    const float b = x == top ? 0.0f : (top - x) * inv;
+    return b < BINS - 1 ? static_cast<int>(b) : BINS - 1;
+}
+// Bins of equal factors in weight, the last one from 2^-32.
+template <int BINS>
+__device__ __forceinline__ float weight_bins(const Weigh& weigh) {
+    return static_cast<float>(fmin(weigh.c * (BINS / 32.0 / kRoots), 3e38));
+}
+
+// A lane a run of the row, `sum` its kept weight: the first run whose running
+// sum passes draw times the total (the last with any weight where rounding
+// leaves none), and what of that is wanted of the run.
+__device__ __forceinline__ int pick_run(double sum, double draw, double& total, double& target) {
+    const double run = wave_scan(sum);
+    total = last_lane(run);
+    target = draw * total;
+    const u64 some = __ballot(sum > 0.0), past = __ballot(sum > 0.0 && run > target);
+    const int pick = past ? __ffsll(past) - 1 : 63 - __clzll(some);
+    target = fmax(0.0, target - __shfl(run - sum, pick, kWave));
+    return pick;
+}
+
+// Draws from logits [begin, end) by the whole workgroup, consecutive ones a
+// thread: those above thr and the first `left` at it, of weight wt, of which
+// `target` is wanted; `total` is the row's.
+template <class Shared, class At, class Kept>
+__device__ __forceinline__ void draw_in_run(const SampleArgs& a, int r, Shared& s, At at,
+                                            int begin, int end, Kept kept, float cut, float thr,
+                                            uint32_t left, double wt, double target, double total) {
+    const int tid = threadIdx.x, span = end - begin;
+    const int each = (span + kSampleThreads - 1) / kSampleThreads;
+    const int from = begin + tid * each, to = min(from + each, end);
+    double mine = 0.0;
+    uint32_t n = 0;
+    for (int p = from; p < to; ++p) {
+        const float x = at(p);
+        if (x > thr && x >= cut) mine += kept(x);
+        n += x == thr && wt > 0.0;
+    }
+    uint32_t here = 0;
+    if (left > 0) {
+        uint32_t all_n = 0;
+        const uint32_t n_before = block_prefix(n, s.part_n, all_n);
+        here = left > n_before ? min(left - n_before, n) : 0;
+        mine += here * wt;
+    }
+    double all = 0.0;
+    const double before = block_prefix(mine, s.part, all);
+    const bool hit = mine > 0.0 && before <= target && before + mine > target;
+    if (hit) s.token = 1;
+    if (mine > 0.0) atomicMax(&s.last, tid);
+    __syncthreads();
+    // The scan's rounding may leave a gap that the target falls into: the
+    // last thread with any weight then takes it.
+    if (!(hit || (s.token < 0 && tid == s.last))) return;
+    double run = before, w_token = 0.0;
+    int token = -1;
+    for (int p = from; p < to; ++p) {
+        const float x = at(p);
+        double w = 0.0;
+        if (x > thr) {
+            if (x >= cut) w = kept(x);
+        } else if (x == thr && here > 0) {
+            --here;
+            w = wt;
+        }
+        if (!(w > 0.0)) continue;
+        token = p;
+        w_token = w;
+        run += w;
+        if (run > target) break;
+    }
+    a.tokens[r] = token;
+    if (a.logprobs) a.logprobs[r] = static_cast<float>(log(w_token / total));
+}
+
+// Draws from the n tokens of the list (keys and positions), all that may be
+// kept among them: ranks them, keeps the highest most_kept, of those what top-p
+// (nucleus) and min-p leave, which are some of the highest ranks too.
+template <class Shared>
+__device__ __forceinline__ void draw_from_list(const SampleArgs& a, int r, Shared& s,
+                                               const Settings& set, const Weigh& weigh, uint32_t n,
+                                               uint32_t most_kept, bool nucleus) {
+    const int tid = threadIdx.x;
+    uint32_t key = 0, rank = 0;
+    int pos = 0;
+    const bool mine = static_cast<uint32_t>(tid) < n;
+    if (mine) {
+        key = s.list[tid];
+        pos = s.list_at[tid];
+#pragma unroll 8
+        for (uint32_t i = 0; i < n; ++i) {
+            const uint32_t o = s.list[i];
+            const int at = s.list_at[i];
+            rank += (o > key) | ((o == key) & (at < pos));
+        }
+    }
+    n = min(n, most_kept);
+    const bool in = mine && rank < n;
+    const float x = key_value(key);
+    const double w = in ? weigh(x) : 0.0;
+    const u64 ww = in ? weigh.whole(x) : 0;
+    if (tid == 0) s.keep = n;
+    __syncthreads();  // the list has been read
+    if (in) {
+        s.weight[rank] = ww;
+        s.list_at[rank] = pos;
+    }
+    __syncthreads();
+    if (in) {
+        u64 before = 0, total = 0;
+#pragma unroll 8
+        for (uint32_t i = 0; i < n; ++i) {
+            const u64 o = s.weight[i];
+            before += i < rank ? o : 0;
+            total += o;
+        }
+        if (nucleus) {
+            const u64 target = max(u64{1}, share_up(total, fmaxf(set.top_p, 0.0f)));
+            if (rank > 0 && before >= target) atomicMin(&s.keep, static_cast<int>(rank));
+        }
+        if (w < set.min_p) atomicMin(&s.keep, static_cast<int>(rank));
+    }
+    __syncthreads();
+    const uint32_t keep = s.keep;
+    if (!in || rank >= keep) return;
+    u64 before = 0, total = 0;
+#pragma unroll 8
+    for (uint32_t i = 0; i < keep; ++i) {
+        const u64 o = s.weight[i];
+        const int at = s.list_at[i];
+        before += at < pos ? o : 0;
+        total += o;
+    }
+    const u64 target = set.draw < 1.0 ? share_down(total, static_cast<float>(set.draw)) : total - 1;
+    if (before <= target && before + ww > target) {
+        a.tokens[r] = pos;
+        if (a.logprobs)
+            a.logprobs[r] = static_cast<float>(log(ldexp(w, a.bits) / static_cast<double>(total)));
+    }
+}
+
+// The last token that top-p keeps, from the list's tokens of the border bin
+// (in_bin): the value, and how many of just that value. left: what is wanted of
+// the bin's weight; the first `ties` of thr alone count, where top-k set them.
+template <class Shared, class InBin>
+__device__ __forceinline__ void nucleus_end(Shared& s, const Weigh& weigh, uint32_t n,
+                                            InBin in_bin, u64 left, float& thr, uint32_t& ties) {
+    const int tid = threadIdx.x;
+    uint32_t mine = 0;
+    u64 w = 0;
+    if (static_cast<uint32_t>(tid) < n) {
+        mine = s.list[tid];
+        w = in_bin(mine) ? weigh.whole(key_value(mine)) : 0;
+        s.weight[tid] = w;
+    }
+    __syncthreads();
+    if (w) {
+        u64 above = 0;
+        uint32_t equal = 0;
+#pragma unroll 8
+        for (uint32_t i = 0; i < n; ++i) {
+            const uint32_t o = s.list[i];
+            const u64 ow = s.weight[i];
+            above += o > mine ? ow : 0;
+            equal += o == mine;
+        }
+        if (ties && key_value(mine) == thr) equal = min(equal, ties);
+        if (above < left && above + equal * w >= left) {
+            s.key = mine;
+            s.ties = static_cast<uint32_t>((left - above + w - 1) / w);
+        }
+    }
+    __syncthreads();
+    thr = key_value(s.key);
+    ties = s.ties;
+}
+
+template <bool HELD, class Shared>
+__device__ __forceinline__ void sample_row(const SampleArgs& a, int r, Shared& s, float* held) {
+    constexpr int kBins = Shared::kBins;
+    constexpr int E = kBins / kSampleThreads;  // bins a thread
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     Row<HELD> row;
     row.held = held;
     row.x = a.logits + r * a.stride;
@@ -273,21 +524,16 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
     row.pre = static_cast<int>(reinterpret_cast<uintptr_t>(row.x) / 4 % 4);
     row.chunks = (a.vocab + row.pre + kSampleWaves * kChunk - 1) / (kSampleWaves * kChunk);
     if (tid < 2 * kRoots) s.roots[tid] = kRoot[tid];
-    const float T = a.temperature ? a.temperature[r] : 1.0f;
-    const bool greedy = !(T > 0.0f);
-    const int k = a.top_k && a.top_k[r] < a.vocab ? max(0, a.top_k[r]) : 0;
-    const float top_p = a.top_p ? a.top_p[r] : 1.0f;
-    const float mp = a.min_p ? a.min_p[r] : 0.0f;
-    const double min_p = mp > 0.0f ? fmin(static_cast<double>(mp), 1.0) : 0.0;
-    const float u = a.u[r];
-    const double draw = u > 0.0f ? fmin(static_cast<double>(u), 1.0) : 0.0;
+    const Settings set(a, r);
+    const float top_p = set.top_p;
+    const int k = set.top_k;
+    const double min_p = set.min_p;
 
     // The maximum, and the least of the threads' maxima.
     float most = -INFINITY;
-    const double c = greedy ? 0.0 : kRoots * 1.4426950408889634074 / T;
     // A long row without a filter is read once: its weights are summed beside
     // the maximum, relative to the thread's own so far.
-    const bool once = !HELD && !greedy && k == 0 && !(top_p < 1.0f) && !(mp > 0.0f);
+    const bool once = !HELD && !set.greedy && k == 0 && !(top_p < 1.0f) && min_p == 0.0;
     double sum = 0.0;
     if (once) {
         __syncthreads();  // the roots
@@ -296,7 +542,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
 #pragma unroll
             for (int i = 0; i < Row<HELD>::U; ++i)
                 m = fmaxf(fmaxf(m, fmaxf(v[i].x, v[i].y)), fmaxf(v[i].z, v[i].w));
-            const Weigh weigh{m, false, static_cast<float>(m - 60.0 * T), c, a.bits, s.roots};
+            Weigh weigh = weigh_of(a, set, m, s.roots);
+            weigh.endless = false;  // +inf: summed again
             if (__ballot(m > most)) sum *= m > most ? weigh(most) : 1.0;
 #pragma unroll
             for (int i = 0; i < Row<HELD>::U; ++i)
@@ -306,7 +553,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
     } else {
         row.template each<true>([&](float x, int) { most = fmaxf(most, x); });
     }
-    float top = wave_max(most), low = -wave_max(-most);
+    float top = wave_top(most), low = -wave_top(-most);
     if (lane == 0) {
         s.part_hi[wave] = top;
         s.part_lo[wave] = low;
@@ -332,7 +579,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
         }
         return;
     }
-    const Weigh weigh{top, top == INFINITY, static_cast<float>(top - 60.0 * T), c, a.bits, s.roots};
+    const Weigh weigh = weigh_of(a, set, top, s.roots);
 
     // The last token kept: value thr, the first `ties` of that value.
     float thr = -INFINITY;
@@ -368,81 +615,17 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
         thr = key_value(prefix);
         return left;
     };
-    // The histogram's bin of x; inv: bins over the range they cover.
-    auto bin_of = [&](float x, float inv) {
-        const float b = x == top ? 0.0f : (top - x) * inv;
-        return b < kBins - 1 ? static_cast<int>(b) : kBins - 1;
-    };
+    auto bin_of = [&](float x, float inv) { return bin_at<kBins>(x, top, inv); };
     // Appends a token to the list (s.n counts past its end too).
     auto append = [&](float x, int pos) {
         const uint32_t i = atomicAdd(&s.n, 1u);
         if (i < kList) {
             s.list[i] = order_key(x);
-            s.list_at[i] = pos;
+            s.list_at[i] = pos - row.pre;
         }
     };
 
-    // Every token that may be kept is in the list: ranks them, keeps the
-    // highest most_kept of them, of those what top-p (nucleus) and min-p leave,
-    // which are some of the highest ranks too, and draws.
-    auto draw_from_list = [&](uint32_t n, uint32_t most_kept, bool nucleus) {
-        uint32_t key = 0, rank = 0;
-        int pos = 0;
-        const bool mine = static_cast<uint32_t>(tid) < n;
-        if (mine) {
-            key = s.list[tid];
-            pos = s.list_at[tid];
-#pragma unroll 8
-            for (uint32_t i = 0; i < n; ++i) {
-                const uint32_t o = s.list[i];
-                rank += o > key || (o == key && s.list_at[i] < pos);
-            }
-        }
-        n = min(n, most_kept);
-        const bool in = mine && rank < n;
-        const float x = key_value(key);
-        const double w = in ? weigh(x) : 0.0;
-        const u64 ww = in ? weigh.whole(x) : 0;
-        if (tid == 0) s.keep = n;
-        __syncthreads();  // the list has been read
-        if (in) {
-            s.weight[rank] = ww;
-            s.list_at[rank] = pos;
-        }
-        __syncthreads();
-        if (in) {
-            u64 before = 0, total = 0;
-#pragma unroll 8
-            for (uint32_t i = 0; i < n; ++i) {
-                const u64 o = s.weight[i];
-                before += i < rank ? o : 0;
-                total += o;
-            }
-            if (nucleus) {
-                const u64 target = max(u64{1}, share_up(total, fmaxf(top_p, 0.0f)));
-                if (rank > 0 && before >= target) atomicMin(&s.keep, static_cast<int>(rank));
-            }
-            if (w < min_p) atomicMin(&s.keep, static_cast<int>(rank));
-        }
-        __syncthreads();
-        const uint32_t keep = s.keep;
-        if (!in || rank >= keep) return;
-        u64 before = 0, total = 0;
-#pragma unroll 8
-        for (uint32_t i = 0; i < keep; ++i) {
-            const u64 o = s.weight[i];
-            before += s.list_at[i] < pos ? o : 0;
-            total += o;
-        }
-        const u64 target = draw < 1.0 ? share_down(total, static_cast<float>(draw)) : total - 1;
-        if (before <= target && before + ww > target) {
-            a.tokens[r] = pos - row.pre;
-            if (a.logprobs)
-                a.logprobs[r] = static_cast<float>(log(ldexp(w, a.bits) / static_cast<double>(total)));
-        }
-    };
-
-    if (greedy) {
+    if (set.greedy) {
         // The lowest index of the maximum.
         int first = 0x7fffffff;
         row.each([&](float x, int pos) { first = x == top ? min(first, pos) : first; });
@@ -463,7 +646,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
         if (low == -INFINITY || k > kSampleThreads) {
             float least = INFINITY;
             row.each([&](float x, int) { least = x > -INFINITY ? fminf(least, x) : least; });
-            least = -wave_max(-least);
+            least = -wave_top(-least);
             __syncthreads();
             if (lane == 0) s.part_lo[wave] = least;
             __syncthreads();
@@ -476,16 +659,24 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
             if (x >= floor) atomicAdd(&s.count[bin_of(x, inv)], 1u);
         });
         __syncthreads();
-        const uint32_t b0 = s.count[2 * tid], b1 = s.count[2 * tid + 1];
-        uint32_t all = 0;
-        const uint32_t want = k, before = block_prefix(b0 + b1, s.part_n, all);
+        uint32_t bins[E], sum_n = 0, all = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            bins[i] = s.count[E * tid + i];
+            sum_n += bins[i];
+        }
+        const uint32_t want = k;
+        uint32_t before = block_prefix(sum_n, s.part_n, all);
         // Fewer tokens than k that can be drawn: the filter is off.
         if (all >= want) {
-            if (before < want && before + b0 + b1 >= want) {
-                const bool second = before + b0 < want;
-                s.bin = 2 * tid + second;
-                s.left = want - before - (second ? b0 : 0);
-                s.bin_end = before + b0 + (second ? b1 : 0);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                if (before < want && before + bins[i] >= want) {
+                    s.bin = E * tid + i;
+                    s.left = want - before;
+                    s.bin_end = before + bins[i];
+                }
+                before += bins[i];
             }
             __syncthreads();
             const int bin = s.bin;
@@ -501,7 +692,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
             __syncthreads();
             const uint32_t n = s.n;
             if (whole) {
-                draw_from_list(n, want, top_p < 1.0f);
+                draw_from_list(a, r, s, set, weigh, n, want, top_p < 1.0f);
                 return;
             }
             if (n <= kList) {
@@ -510,8 +701,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
                     uint32_t above = 0, equal = 0;
 #pragma unroll 8
                     for (uint32_t i = 0; i < n; ++i) {
-                        above += s.list[i] > mine;
-                        equal += s.list[i] == mine;
+                        const uint32_t o = s.list[i];
+                        above += o > mine;
+                        equal += o == mine;
                     }
                     if (above < left && above + equal >= left) {
                         s.key = mine;
@@ -533,39 +725,60 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
             __syncthreads();
         } else {
             __syncthreads();
-            s.count[2 * tid] = s.count[2 * tid + 1] = 0;
+            for (int i = tid; i < kBins; i += kSampleThreads) s.count[i] = 0;
             __syncthreads();
         }
     }
 
     if (top_p < 1.0f) {
-        // Bins of 1/64 of a factor of two in weight, the last one from 2^-32.
-        const float inv = static_cast<float>(fmin(weigh.c * (64.0 / kRoots), 3e38));
+        const float inv = weight_bins<kBins>(weigh);
+        // The last bin holds most of a row at a low temperature: one add a thread.
+        u64 rest = 0;
+        uint32_t rest_n = 0;
         row.each([&](float x, int) {
             if (x > thr && x >= weigh.least) {
                 const int b = bin_of(x, inv);
-                atomicAdd(&s.weight[b], weigh.whole(x));
-                atomicAdd(&s.count[b], 1u);
+                const u64 w = weigh.whole(x);
+                if (b == kBins - 1) {
+                    rest += w;
+                    ++rest_n;
+                } else {
+                    atomicAdd(&s.weight[b], w);
+                    atomicAdd(&s.count[b], 1u);
+                }
             }
         });
+        if (rest_n) {
+            atomicAdd(&s.weight[kBins - 1], rest);
+            atomicAdd(&s.count[kBins - 1], rest_n);
+        }
         if (tid == 0 && ties) {
             const int b = bin_of(thr, inv);
             atomicAdd(&s.weight[b], ties * weigh.whole(thr));
             atomicAdd(&s.count[b], ties);
         }
         __syncthreads();
-        const u64 b0 = s.weight[2 * tid], b1 = s.weight[2 * tid + 1];
-        const uint32_t n0 = s.count[2 * tid], n1 = s.count[2 * tid + 1];
-        u64 total = 0;
-        uint32_t all = 0;
-        const u64 before = block_prefix(b0 + b1, s.part64, total);
-        const uint32_t n_before = block_prefix(n0 + n1, s.part_n, all);
+        u64 bins[E], sum_w = 0, total = 0;
+        uint32_t counts[E], sum_n = 0, all = 0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            bins[i] = s.weight[E * tid + i];
+            counts[i] = s.count[E * tid + i];
+            sum_w += bins[i];
+            sum_n += counts[i];
+        }
+        u64 before = block_prefix(sum_w, s.part64, total);
+        uint32_t n_before = block_prefix(sum_n, s.part_n, all);
         const u64 target = max(u64{1}, share_up(total, fmaxf(top_p, 0.0f)));
-        if (before < target && before + b0 + b1 >= target) {
-            const bool second = before + b0 < target;
-            s.bin = 2 * tid + second;
-            s.left = target - before - (second ? b0 : 0);
-            s.bin_end = n_before + n0 + (second ? n1 : 0);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            n_before += counts[i];
+            if (before < target && before + bins[i] >= target) {
+                s.bin = E * tid + i;
+                s.left = target - before;
+                s.bin_end = n_before;
+            }
+            before += bins[i];
         }
         __syncthreads();
         const int bin = s.bin;
@@ -580,40 +793,14 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
         __syncthreads();
         const uint32_t n = s.n;
         if (n <= kList) {
-            uint32_t mine = 0;
-            u64 w = 0;
-            if (static_cast<uint32_t>(tid) < n) {
-                mine = s.list[tid];
-                w = weigh.whole(key_value(mine));
-                s.weight[tid] = w;
-            }
-            __syncthreads();
-            // In the border bin: a token's weight counts from the bins above.
-            if (static_cast<uint32_t>(tid) < n && bin_of(key_value(mine), inv) == bin && w) {
-                u64 above = 0;
-                uint32_t equal = 0;
-#pragma unroll 8
-                for (uint32_t i = 0; i < n; ++i) {
-                    const bool here = !whole || bin_of(key_value(s.list[i]), inv) == bin;
-                    above += here && s.list[i] > mine ? s.weight[i] : 0;
-                    equal += s.list[i] == mine;
-                }
-                if (ties && key_value(mine) == thr) equal = min(equal, ties);
-                if (above < left && above + equal * w >= left) {
-                    s.key = mine;
-                    s.ties = static_cast<uint32_t>((left - above + w - 1) / w);
-                }
-            }
-            __syncthreads();
-            thr = key_value(s.key);
-            ties = s.ties;
+            nucleus_end(s, weigh, n, [&](uint32_t key) { return bin_of(key_value(key), inv) == bin; },
+                        left, thr, ties);
             if (whole) {
                 // What stays of the list: those above the last kept, and it.
                 uint32_t above = 0;
                 if (static_cast<uint32_t>(tid) < n) above = s.list[tid] > s.key;
-                uint32_t kept_above = 0;
-                (void)block_prefix(above, s.part_n, kept_above);
-                draw_from_list(n, kept_above + ties, false);
+                const uint32_t kept_above = __syncthreads_count(above);
+                draw_from_list(a, r, s, set, weigh, n, kept_above + ties, false);
                 return;
             }
         } else {
@@ -623,11 +810,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
         }
     }
 
-    // No logit below `cut` weighs min_p (a thousandth of T and the fp32
-    // roundings of the sum are left for the comparison in 64 bits).
-    const float cut = weigh.endless ? -INFINITY : min_p > 0.0 ? static_cast<float>(top + (log(min_p) - 1e-3) * T -
-                                                       1e-6 * fabs(static_cast<double>(top)))
-                                  : weigh.least;
+    const float cut = cut_of(set, weigh);
     auto kept = [&](float x) {  // the weight of a token that top-k and top-p keep
         const double w = weigh(x);
         return w >= min_p ? w : 0.0;
@@ -645,101 +828,427 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
             at_thr += x == thr && ties;
         });
     }
-    sum = __shfl(wave_scan(sum), kWave - 1, kWave);
-    at_thr = __shfl(wave_scan(at_thr), kWave - 1, kWave);
+    sum = last_lane(wave_scan(sum));
+    at_thr = last_lane(wave_scan(at_thr));
     __syncthreads();
     if (lane == 0) {
         s.part[wave] = sum;
         s.part_n[wave] = at_thr;
     }
     __syncthreads();
-    double total = 0.0;
-    {
-        uint32_t left = ties;
-#pragma unroll
-        for (int i = 0; i < kSampleWaves; ++i) {
-            const uint32_t n = min(left, s.part_n[i]);
-            left -= n;
-            total += s.part[i] + n * wt;
-        }
-    }
-    double target = draw * total;
-    int pick = 0;
-    uint32_t left = ties;
-    {
-        // The first wave whose running sum passes the target (the last with
-        // any weight where rounding leaves none).
-        double run = 0.0, pick_run = 0.0;
-        uint32_t l = ties;
-        bool found = false;
-#pragma unroll
-        for (int i = 0; i < kSampleWaves; ++i) {
-            const uint32_t n = min(l, s.part_n[i]);
-            const double w = s.part[i] + n * wt;
-            if (!found && w > 0.0) {
-                pick = i;
-                pick_run = run;
-                left = l;
-                found = run + w > target;
-            }
-            l -= n;
-            run += w;
-        }
-        target -= pick_run;
-    }
-    // That wave's run of the row, `each` consecutive logits a thread.
-    const int span = row.chunks * kChunk, each = (span + kSampleThreads - 1) / kSampleThreads;
-    const int from = pick * span + tid * each, to = min(from + each, (pick + 1) * span);
-    double mine = 0.0;
-    uint32_t n = 0;
-    for (int p = from; p < to; ++p) {
-        const float x = row.at(p);
-        if (x > thr && x >= cut) mine += kept(x);
-        n += x == thr && ties;
-    }
-    uint32_t all_n = 0;
-    const uint32_t n_before = block_prefix(n, s.part_n, all_n);
-    uint32_t here = left > n_before ? min(left - n_before, n) : 0;
-    mine += here * wt;
-    double all = 0.0;
-    const double before = block_prefix(mine, s.part, all);
-    const bool hit = mine > 0.0 && before <= target && before + mine > target;
-    if (hit) s.token = 1;
-    if (mine > 0.0) atomicMax(&s.last, tid);
-    __syncthreads();
-    // The scan's rounding may leave a gap that the target falls into: the
-    // last thread with any weight then takes it.
-    if (!(hit || (s.token < 0 && tid == s.last))) return;
-    double run = before;
-    int token = -1;
-    double w_token = 0.0;
-    for (int p = from; p < to; ++p) {
-        const float x = row.at(p);
-        double w = 0.0;
-        if (x > thr) {
-            if (x >= cut) w = kept(x);
-        } else if (x == thr && here > 0) {
-            --here;
-            w = wt;
-        }
-        if (!(w > 0.0)) continue;
-        token = p - row.pre;
-        w_token = w;
-        run += w;
-        if (run > target) break;
-    }
-    a.tokens[r] = token;
-    if (a.logprobs) a.logprobs[r] = static_cast<float>(log(w_token / total));
+    // The first wave whose running sum passes the target (the last with any
+    // weight where rounding leaves none), a lane a wave.
+    const bool is_wave = lane < kSampleWaves;
+    const uint32_t n_here = is_wave ? s.part_n[lane] : 0, n_before = wave_scan(n_here) - n_here;
+    const uint32_t n_kept = min(n_here, ties - min(ties, n_before));
+    double total = 0.0, target = 0.0;
+    const int pick = pick_run(is_wave ? s.part[lane] + n_kept * wt : 0.0, set.draw, total, target);
+    const uint32_t left = ties - min(ties, __shfl(n_before, pick, kWave));
+    // Of that wave's run of the row, positions as indexes.
+    const int span = row.chunks * kChunk;
+    draw_in_run(a, r, s, [&](int i) { return row.at(i + row.pre); }, max(0, pick * span - row.pre),
+                min(a.vocab, (pick + 1) * span - row.pre), kept, cut, thr, left, wt, target, total);
 }
 
-std::size_t sample_scratch(std::size_t, std::size_t) { return 0; }
+template <bool HELD>
+__global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a) {
+    __shared__ SampleShared<HELD ? kHeldBins : kWideBins> s;
+    extern __shared__ __attribute__((aligned(16))) float held[];
+    sample_row<HELD>(a, blockIdx.x, s, held);
+}
 
-void run_sample(const SampleArgs& a, hipStream_t stream) {
-    // Rows that fit LDS beside the rest, up to three floats off their 16 bytes.
-    const int per = kSampleWaves * kChunk, chunks = (a.vocab + 3 + per - 1) / per;
+// --- few rows of a large vocabulary: a row over several workgroups ------------------
+//
+// The same steps, a launch each, every row in slices of consecutive logits
+// (blockIdx.x, a workgroup of 256 threads each), the histograms added up in
+// the caller's scratch by integer atomics, and a last launch of one workgroup a
+// row that draws. Rows that this does not fit (a logit of +inf, a border bin of
+// more than kList) are done by that workgroup alone, as above. Calls without
+// top-k only.
+
+constexpr int kMaxSlices = 32;
+constexpr int kSliceThreads = 256;
+
+struct SliceRow {
+    u64 weight[kWideBins];
+    uint32_t count[kWideBins];
+    double sum[kMaxSlices];  // kept weights, but for the border bin's
+    float top[kMaxSlices];
+    int first[kMaxSlices];  // lowest index of the slice's maximum
+    uint32_t list[kList];
+    int list_at[kList];
+    uint32_t n, pad[3];
+};
+
+struct SliceArgs {
+    SampleArgs a;
+    SliceRow* rows;
+    int slices, length;
+};
+
+enum RowKind { kNothing, kGreedy, kPlain, kTopP, kAlone };
+
+// What the slices' maxima say of the row.
+struct SliceView {
+    float top;
+    int first;
+    RowKind kind;
+    // By wave: a lane a slice, so that the loads are in flight together.
+    __device__ SliceView(const SliceArgs& b, const SliceRow& row, const Settings& set) {
+        const int i = min(static_cast<int>(threadIdx.x % kWave), b.slices - 1);
+        const float t = row.top[i];
+        top = wave_top(t);
+        first = wave_least(t == top ? row.first[i] : 0x7fffffff);
+        kind = top == -INFINITY  ? kNothing
+               : set.greedy      ? kGreedy
+               : top == INFINITY ? kAlone
+               : set.top_p < 1.0f ? kTopP
+                                  : kPlain;
+    }
+};
+
+// The slice's maximum; clears the row's histogram.
+__global__ __launch_bounds__(kSliceThreads) void slice_top_kernel(SliceArgs b) {
+    __shared__ float hi[kSliceThreads / kWave];
+    __shared__ int at[kSliceThreads / kWave];
+    const int s = blockIdx.x, r = blockIdx.y, tid = threadIdx.x, lane = tid % kWave;
+    const float* x = b.a.logits + r * b.a.stride;
+    SliceRow& row = b.rows[r];
+    const int begin = s * b.length, end = min(begin + b.length, b.a.vocab);
+    float top = -INFINITY;
+    int first = 0x7fffffff;
+#pragma unroll 8
+    for (int i = begin + tid; i < end; i += kSliceThreads) {
+        const float v = clean(x[i]);
+        first = v > top ? i : first;
+        top = fmaxf(top, v);
+    }
+    float m = wave_top(top);
+    int f = top == m ? first : 0x7fffffff;
+    f = wave_least(f);
+    if (lane == 0) {
+        hi[tid / kWave] = m;
+        at[tid / kWave] = f;
+    }
+    for (int i = s * kSliceThreads + tid; i < kWideBins; i += b.slices * kSliceThreads) {
+        row.weight[i] = 0;
+        row.count[i] = 0;
+    }
+    if (s == 0 && tid == 0) row.n = 0;
+    __syncthreads();
+    if (tid == 0) {
+        for (int i = 1; i < kSliceThreads / kWave; ++i) {
+            if (hi[i] > m || (hi[i] == m && at[i] < f)) f = at[i];
+            m = fmaxf(m, hi[i]);
+        }
+        row.top[s] = m;
+        row.first[s] = f;
+    }
+}
+
+__device__ __forceinline__ double block_sum64(double v, double* part) {
+    v = last_lane(wave_scan(v));
+    if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = v;
+    __syncthreads();
+    return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// The slice's part of the row's histogram, or the sum of its weights.
+__global__ __launch_bounds__(kSliceThreads) void slice_count_kernel(SliceArgs b) {
+    __shared__ u64 weight[kWideBins];
+    __shared__ uint32_t count[kWideBins];
+    __shared__ double roots[2 * kRoots];
+    __shared__ double part[kSliceThreads / kWave];
+    const int s = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+    const SampleArgs& a = b.a;
+    SliceRow& row = b.rows[r];
+    const Settings set(a, r);
+    const SliceView view(b, row, set);
+    if (view.kind == kNothing || view.kind == kGreedy || view.kind == kAlone) return;
+    if (tid < 2 * kRoots) roots[tid] = kRoot[tid];
+    for (int i = tid; i < kWideBins; i += kSliceThreads) {
+        weight[i] = 0;
+        count[i] = 0;
+    }
+    __syncthreads();
+    const Weigh weigh = weigh_of(a, set, view.top, roots);
+    const float* x = a.logits + r * a.stride;
+    const int begin = s * b.length, end = min(begin + b.length, a.vocab);
+    if (view.kind == kPlain) {
+        const float cut = cut_of(set, weigh);
+        double sum = 0.0;
+#pragma unroll 4
+        for (int i = begin + tid; i < end; i += kSliceThreads) {
+            const float v = clean(x[i]);
+            if (v >= cut) {
+                const double w = weigh(v);
+                sum += w >= set.min_p ? w : 0.0;
+            }
+        }
+        sum = block_sum64(sum, part);
+        if (tid == 0) row.sum[s] = sum;
+        return;
+    }
+    const float inv = weight_bins<kWideBins>(weigh);
+    u64 rest = 0;  // the last bin's, one add a thread
+    uint32_t rest_n = 0;
+#pragma unroll 4
+    for (int i = begin + tid; i < end; i += kSliceThreads) {
+        const float v = clean(x[i]);
+        if (v >= weigh.least) {
+            const int bin = bin_at<kWideBins>(v, view.top, inv);
+            const u64 w = weigh.whole(v);
+            if (bin == kWideBins - 1) {
+                rest += w;
+                ++rest_n;
+            } else {
+                atomicAdd(&weight[bin], w);
+                atomicAdd(&count[bin], 1u);
+            }
+        }
+    }
+    if (rest_n) {
+        atomicAdd(&weight[kWideBins - 1], rest);
+        atomicAdd(&count[kWideBins - 1], rest_n);
+    }
+    __syncthreads();
+    for (int i = tid; i < kWideBins; i += kSliceThreads) {
+        if (!count[i]) continue;
+        atomicAdd(&row.count[i], count[i]);
+        if (weight[i]) atomicAdd(&row.weight[i], weight[i]);
+    }
+}
+
+// The bin at which top-p ends, from the row's histogram, by a
+// workgroup of THREADS.
+struct Border {
+    int bin;
+    uint32_t count;  // tokens up to and with the bin
+    u64 left;        // what is wanted of the bin's weight
+};
+template <int THREADS>
+__device__ __forceinline__ Border border_of(const SliceRow& row, const Settings& set, u64* part,
+                                            Border* out) {
+    constexpr int E = kWideBins / THREADS;
+    const int tid = threadIdx.x, wave = tid / kWave;
+    u64 w[E], sum = 0;
+    uint32_t n[E], all = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        n[i] = row.count[E * tid + i];
+        w[i] = row.weight[E * tid + i];
+        sum += w[i];
+        all += n[i];
+    }
+    const u64 scan = wave_scan(sum);
+    const uint32_t scan_n = wave_scan(all);
+    if (tid % kWave == kWave - 1) {
+        part[2 * wave] = scan;
+        part[2 * wave + 1] = scan_n;
+    }
+    __syncthreads();
+    u64 before = scan - sum, total = 0;
+    uint32_t count = scan_n - all;
+#pragma unroll
+    for (int i = 0; i < THREADS / kWave; ++i) {
+        before += i < wave ? part[2 * i] : 0;
+        count += i < wave ? static_cast<uint32_t>(part[2 * i + 1]) : 0;
+        total += part[2 * i];
+    }
+    const u64 target = max(u64{1}, share_up(total, fmaxf(set.top_p, 0.0f)));
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        count += n[i];
+        if (before < target && before + w[i] >= target) *out = Border{E * tid + i, count, target - before};
+        before += w[i];
+    }
+    __syncthreads();
+    return *out;
+}
+
+// The tokens of the border bin, or of all bins up to it where they are few;
+// the sum of the slice's weights above it.
+__global__ __launch_bounds__(kSliceThreads) void slice_list_kernel(SliceArgs b) {
+    __shared__ double roots[2 * kRoots];
+    __shared__ double part[kSliceThreads / kWave];
+    __shared__ u64 part64[2 * kSliceThreads / kWave];
+    __shared__ Border border;
+    const int s = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+    const SampleArgs& a = b.a;
+    SliceRow& row = b.rows[r];
+    const Settings set(a, r);
+    const SliceView view(b, row, set);
+    if (view.kind != kTopP) return;
+    if (tid < 2 * kRoots) roots[tid] = kRoot[tid];
+    const Border end_at = border_of<kSliceThreads>(row, set, part64, &border);
+    const Weigh weigh = weigh_of(a, set, view.top, roots);
+    const bool whole = end_at.count <= kShort;
+    const float inv = weight_bins<kWideBins>(weigh), cut = cut_of(set, weigh);
+    const float* x = a.logits + r * a.stride;
+    const int begin = s * b.length, end = min(begin + b.length, a.vocab);
+    double sum = 0.0;
+#pragma unroll 4
+    for (int i = begin + tid; i < end; i += kSliceThreads) {
+        const float v = clean(x[i]);
+        if (!(v >= weigh.least)) continue;
+        const int bin = bin_at<kWideBins>(v, view.top, inv);
+        if (bin == end_at.bin || (whole && bin < end_at.bin)) {
+            const uint32_t n = atomicAdd(&row.n, 1u);
+            if (n < kList) {
+                row.list[n] = order_key(v);
+                row.list_at[n] = i;
+            }
+        } else if (bin < end_at.bin && v >= cut) {
+            const double w = weigh(v);
+            sum += w >= set.min_p ? w : 0.0;
+        }
+    }
+    sum = block_sum64(sum, part);
+    if (tid == 0) row.sum[s] = sum;
+}
+
+__global__ __launch_bounds__(kSampleThreads) void slice_draw_kernel(SliceArgs b) {
+    __shared__ SampleShared<kWideBins> s;
+    __shared__ Border border;
+    const SampleArgs& a = b.a;
+    const int r = blockIdx.x, tid = threadIdx.x;
+    const SliceRow& row = b.rows[r];
+    const Settings set(a, r);
+    const SliceView view(b, row, set);
+    if (view.kind == kNothing || view.kind == kGreedy) {
+        if (tid == 0) {
+            a.tokens[r] = view.kind == kGreedy ? view.first : -1;
+            if (a.logprobs) a.logprobs[r] = view.kind == kGreedy ? 0.0f : -INFINITY;
+        }
+        return;
+    }
+    bool alone = view.kind == kAlone;
+    Border end_at{};
+    uint32_t n = 0;
+    if (view.kind == kTopP) {
+        end_at = border_of<kSampleThreads>(row, set, s.part64, &border);
+        n = row.n;
+        alone = n > kList;
+    }
+    if (alone) {
+        __syncthreads();
+        sample_row<false>(a, r, s, nullptr);
+        return;
+    }
+    if (tid < 2 * kRoots) s.roots[tid] = kRoot[tid];
+    if (tid == 0) s.token = s.last = -1;
+    if (static_cast<uint32_t>(tid) < n) {
+        s.list[tid] = row.list[tid];
+        s.list_at[tid] = row.list_at[tid];
+    }
+    __syncthreads();
+    const Weigh weigh = weigh_of(a, set, view.top, s.roots);
+    float thr = -INFINITY;
+    uint32_t ties = 0;
+    const float cut = cut_of(set, weigh);
+    auto kept = [&](float v) {
+        const double w = weigh(v);
+        return w >= set.min_p ? w : 0.0;
+    };
+    if (view.kind == kTopP) {
+        const float inv = weight_bins<kWideBins>(weigh);
+        nucleus_end(s, weigh, n,
+                    [&](uint32_t key) { return bin_at<kWideBins>(key_value(key), view.top, inv) == end_at.bin; },
+                    end_at.left, thr, ties);
+        // The list by rank, so that the sums do not depend on its order.
+        uint32_t key = 0, rank = 0, above = 0;
+        int pos = 0;
+        if (static_cast<uint32_t>(tid) < n) {
+            key = s.list[tid];
+            pos = s.list_at[tid];
+            above = key > s.key;
+#pragma unroll 8
+            for (uint32_t i = 0; i < n; ++i) {
+                const uint32_t o = s.list[i];
+                const int at = s.list_at[i];
+                rank += (o > key) | ((o == key) & (at < pos));
+            }
+        }
+        const uint32_t kept_above = __syncthreads_count(above);
+        if (end_at.count <= kShort) {
+            draw_from_list(a, r, s, set, weigh, n, kept_above + ties, false);
+            return;
+        }
+        n = kept_above + ties;  // of the list, by rank
+        __syncthreads();  // the list has been read
+        if (key && rank < n) {
+            s.list_at[rank] = pos;
+            s.weight[rank] = __double_as_longlong(kept(key_value(key)));
+        }
+        __syncthreads();
+    }
+    const double wt = ties ? kept(thr) : 0.0;
+    // Slice sums with the list's kept tokens, a wave a slice, in a fixed pattern.
+    for (int i = tid / kWave; i < b.slices; i += kSampleWaves) {
+        const int begin = i * b.length, end = begin + b.length;
+        double sum = 0.0;
+        for (uint32_t y = tid % kWave; y < n; y += kWave) {
+            const int at = s.list_at[y];
+            sum += at >= begin && at < end ? __longlong_as_double(s.weight[y]) : 0.0;
+        }
+        sum = last_lane(wave_scan(sum));
+        if (tid % kWave == 0) s.sums[i] = row.sum[i] + sum;
+    }
+    __syncthreads();
+    double total = 0.0, target = 0.0;
+    const int lane = tid % kWave;
+    const int pick = pick_run(lane < b.slices ? s.sums[lane] : 0.0, set.draw, total, target);
+    const int begin = pick * b.length;
+    // Tokens at the threshold that slices before this one keep.
+    uint32_t left = ties;
+    if (ties)
+        for (uint32_t i = n - ties; i < n; ++i) left -= s.list_at[i] < begin;
+    const float* x = a.logits + r * a.stride;
+    draw_in_run(a, r, s, [&](int i) { return clean(x[i]); }, begin, min(begin + b.length, a.vocab), kept,
+                cut, thr, left, wt, target, total);
+}
+
+// Chunks a wave of the row kernel, for a row up to three floats off its 16 bytes.
+int row_chunks(std::size_t vocab) {
+    return ceil_div(static_cast<long long>(vocab) + 3, kSampleWaves * kChunk);
+}
+
+// Slices a row takes, 1: the row kernel, which has rows that LDS holds and many
+// of them. us, row kernel / slices, top-p of 0.9: 1 x 32000 38 / 37, 1 x 50000
+// 60 / 38, 32 x 50000 62 / 63, 1 x 100003 106 / 46, 7 x 100003 107 / 51, 32 x
+// 100003 107 / 77, 64 x 100003 107 / 111; no filter: 41 / 21 at 1 x 100003, 25 /
+// 28 at 64 x 50000. Not with a top-k, which leaves the row kernel little to do
+// after its histogram: 39 / 48 at 7 x 100003, 15 / 27 at 1 x 32000.
+int slices_of(std::size_t rows, std::size_t vocab) {
+    if (row_chunks(vocab) <= kHeldChunks || rows > vocab / 2048) return 1;
+    return static_cast<int>(std::min<std::size_t>({kMaxSlices, vocab / 2048, 512 / rows}));
+}
+
+std::size_t sample_scratch(std::size_t rows, std::size_t vocab) {
+    return slices_of(rows, vocab) > 1 ? rows * sizeof(SliceRow) : 0;
+}
+
+void run_slices(const SampleArgs& a, int slices, void* scratch, hipStream_t stream) {
+    SliceArgs b{a, static_cast<SliceRow*>(scratch), slices, 0};
+    b.length = (ceil_div(a.vocab, slices) + kSliceThreads - 1) / kSliceThreads * kSliceThreads;
+    b.slices = ceil_div(a.vocab, b.length);
+    const dim3 grid(b.slices, a.rows), block(kSliceThreads);
+    hipLaunchKernelGGL(slice_top_kernel, grid, block, 0, stream, b);
+    hipLaunchKernelGGL(slice_count_kernel, grid, block, 0, stream, b);
+    if (a.top_p) hipLaunchKernelGGL(slice_list_kernel, grid, block, 0, stream, b);
+    hipLaunchKernelGGL(slice_draw_kernel, dim3(a.rows), dim3(kSampleThreads), 0, stream, b);
+}
+
+void run_sample(const SampleArgs& a, void* scratch, hipStream_t stream) {
+    const int slices = slices_of(static_cast<std::size_t>(a.rows), static_cast<std::size_t>(a.vocab));
+    if (slices > 1 && !a.top_k) {
+        run_slices(a, slices, scratch, stream);
+        return;
+    }
+    const int chunks = row_chunks(static_cast<std::size_t>(a.vocab));
     if (chunks <= kHeldChunks)
         hipLaunchKernelGGL(sample_row_kernel<true>, dim3(a.rows), dim3(kSampleThreads),
-                           chunks * per * sizeof(float), stream, a);
+                           chunks * kSampleWaves * kChunk * sizeof(float), stream, a);
     else
         hipLaunchKernelGGL(sample_row_kernel<false>, dim3(a.rows), dim3(kSampleThreads), 0, stream, a);
 }
@@ -788,7 +1297,7 @@ int em_sample(size_t rows, size_t vocab, const float* logits, size_t logits_stri
         a.min_p = settings->min_p;
         a.tokens = tokens;
         a.logprobs = logprobs;
-        em::run_sample(a, static_cast<hipStream_t>(stream));
+        em::run_sample(a, scratch, static_cast<hipStream_t>(stream));
         em::hip_check(hipGetLastError(), "launch");
     } catch (const std::exception& e) {
         return fail(EM_EDEVICE, e.what());

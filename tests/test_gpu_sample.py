@@ -220,3 +220,64 @@ def test_python_checks():
                dict(tokens=u), dict(scratch=u)):
         with pytest.raises(em.InvalidArgument):
             em.sample(**{**dict(logits=x, u=u), **kw})
+
+
+# Rows that are spread over workgroups (few of a large vocabulary), rows done by
+# one workgroup from memory (many) and from LDS (up to 32765 logits).
+SPREADS = [(1, 9000), (3, 20000), (2, 50021), (100, 40007), (300, 33000), (200, 30000)]
+
+
+@pytest.mark.parametrize("R, V", SPREADS)
+def test_masked_runs_and_every_setting(R, V):
+    """Long runs of -inf and NaN, where whole threads have nothing to draw."""
+    rng = np.random.default_rng(R * V)
+    R = min(R, 100) if V > 35000 else R
+    x = logits(R, V, rng, 1.5)
+    x[:, V // 4:V // 2] = -np.inf
+    x[0, :] = -np.inf
+    x[0, [3, V // 2 + 7, V - 1]] = [1.0, 2.0, 0.5]
+    if R > 2:
+        x[1, V // 2:] = np.nan
+        x[2, :-2] = -np.inf
+    u = rng.random(R).astype(np.float32)
+    step = max(1, R // 12)
+    x, u = x[::step].copy(), u[::step].copy()
+    x = np.concatenate([x, np.repeat(x[-1:], R - x.shape[0], 0)])
+    u = np.concatenate([u, np.repeat(u[-1:], R - u.shape[0], 0)])
+    for kw in (dict(), dict(T=0.0), dict(T=math.inf), dict(T=0.2, p=0.9), dict(T=5.0, p=0.5),
+               dict(k=40), dict(k=128, p=0.9), dict(k=129), dict(k=2000, p=0.3, mp=0.01),
+               dict(p=0.99, mp=0.02), dict(mp=0.3), dict(p=0.0), dict(T=1e-3, p=0.999)):
+        check(x, u, settings(R, rng, **kw))
+
+
+@pytest.mark.parametrize("R, V", [(5, 40000), (300, 40000)])
+def test_ties_across_workgroups(R, V):
+    """Runs of equal logits over the borders between the workgroups' shares."""
+    rng = np.random.default_rng(V + R)
+    x = np.full((R, V), -2.0, np.float32)
+    x[:, ::7] = 1.0
+    x[0] = rng.integers(0, 40, V) * 0.25
+    x[1, 10000:30000] = 3.0
+    x[-1] = 0.5
+    u = rng.random(R).astype(np.float32)
+    u[-1] = 0.99999
+    n = 4  # rows of their own; the rest repeat
+    x[n:-1] = x[2]
+    u[n:-1] = u[2]
+    for kw in (dict(), dict(T=0.0), dict(k=3), dict(k=100), dict(k=5000), dict(p=0.5), dict(p=0.9),
+               dict(k=6000, p=0.7), dict(mp=0.5)):
+        check(x, u, settings(R, rng, **kw))
+
+
+def test_rows_together_or_alone_agree():
+    """A row's draw does not depend on how many rows share the call."""
+    rng = np.random.default_rng(11)
+    x = np.repeat(logits(4, 60013, rng), 100, 0)
+    u = np.tile(rng.random(100).astype(np.float32), 4)
+    p = np.full(400, 0.8, np.float32)
+    many = em.sample(torch.from_numpy(x).cuda(), torch.from_numpy(u).cuda(),
+                     top_p=torch.from_numpy(p).cuda())[0].cpu()
+    for r in (0, 57, 123, 250, 399):
+        one = em.sample(torch.from_numpy(x[r:r + 1]).cuda(), torch.from_numpy(u[r:r + 1]).cuda(),
+                        top_p=torch.from_numpy(p[:1]).cuda())[0].cpu()
+        assert int(one[0]) == int(many[r])
