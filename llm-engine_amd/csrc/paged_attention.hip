@@ -330,6 +330,11 @@ __device__ __forceinline__ uint32_t slot_unit(const PagedArgs& p, int seq, int t
     return off < 0 ? kNoSlot : static_cast<uint32_t>(off >> 3);
 }
 
+template <class T>
+struct __attribute__((aligned(16))) Eight {
+    T v[8];
+};
+
 // One wave, one column over positions lo .. lo + width - 1 of every stride
 // before hi, in fp32 operations on what the column sees alone: for columns
 // whose operands the terms do not hold, and for those beside a position that
@@ -360,7 +365,11 @@ __device__ __forceinline__ void plain_column(const PagedAttnArgs& a, int seq, in
         if (unit != kNoSlot) {
             const T* k = kc + static_cast<std::size_t>(unit) * 8;
             float dot = 0.0f;
-            for (int d = 0; d < D; ++d) dot = fmaf(q[d], static_cast<float>(k[d]), dot);
+            for (int d = 0; d < D; d += 8) {
+                const auto y = *reinterpret_cast<const Eight<T>*>(k + d);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) dot = fmaf(q[d + e], static_cast<float>(y.v[e]), dot);
+            }
             x = dot * a.scale2;
         }
         const float mn = fmaxf(m, wave_max(x));
@@ -370,15 +379,25 @@ __device__ __forceinline__ void plain_column(const PagedAttnArgs& a, int seq, in
         l = l * alpha + wave_sum(w);
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i] *= alpha;
-        for (int i = 0; i < width; ++i) {
-            const uint32_t u = __shfl(unit, i, kWave);
-            if (u == kNoSlot) continue;
-            const float wi = __shfl(w, i, kWave);
-            const T* v = vc + static_cast<std::size_t>(u) * 8;
+        // Eight positions' values in flight; those not seen read slot 0 and count
+        // for nothing, whatever it holds.
+        for (int i = 0; i < width; i += 8) {
+            float v[8][N], wi[8];
 #pragma unroll
-            for (int n = 0; n < N; ++n)
-                if (lane + kWave * n < D)
-                    o[n] = fmaf(wi, static_cast<float>(v[lane + kWave * n]), o[n]);
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t u = __shfl(unit, i + e, kWave);
+                wi[e] = __shfl(w, i + e, kWave);
+                const T* src = vc + static_cast<std::size_t>(u == kNoSlot ? 0 : u) * 8;
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    const float y = static_cast<float>(src[min(lane + kWave * n, D - 1)]);
+                    v[e][n] = u == kNoSlot ? 0.0f : y;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int n = 0; n < N; ++n) o[n] = fmaf(wi[e], v[e][n], o[n]);
         }
     }
 }
