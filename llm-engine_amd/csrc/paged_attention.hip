@@ -697,7 +697,7 @@ __device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& 
         u = units(t0);
         load_k(u);
         load_v(u, v);
-        if constexpr (KT == 3) {
+        if constexpr (KT == 3 && DP <= 128) {
             Raw8<T> v2[NE][NV];
             while (step(v, v2, std::true_type{}) && step(v2, v, std::true_type{})) {
             }
@@ -799,7 +799,7 @@ struct Wide {
     static constexpr int kRowBytes = DP * 2, kPlane = kStep * kRowBytes;
     static constexpr int kStage = 2 * KT * kPlane;  // keys' planes, then values'
     static constexpr int kBufs = 2 * kStage <= 64 * 1024 || KT == 3 ? (KT == 3 && DP > 64 ? 1 : 2) : 1;
-    static constexpr bool kQueryLds = NT == 3 && DP <= 128;
+    static constexpr bool kQueryLds = NT == 3;
     static constexpr int kQueryAt = kBufs * kStage;
     static constexpr int kLds = kQueryAt + (kQueryLds ? kWaves * C * kWave * 16 : 0);
     static_assert(kWaves * 32 * (8 * DU + 4) * 4 <= kLds);
@@ -1248,7 +1248,8 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, i
 
 // --- launch ---------------------------------------------------------------------------
 
-int paged_slots() { return 2 * cu_count(); }
+// Workgroups the card holds at once: heads past 128 take a CU's registers.
+int paged_slots(const em_paged_shape& s) { return (s.head_size <= 128 ? 2 : 1) * cu_count(); }
 
 // Whether any sequence of the shape can be split: it needs one and a half
 // runs' positions.
@@ -1268,7 +1269,7 @@ bool can_widen(const em_paged_shape& s, std::size_t rows) {
 // for the float arithmetic of the plan.
 int partial_units(const em_paged_shape& s, std::size_t rows) {
     if (!can_split(s)) return 0;
-    return (paged_slots() * 17 / 12 + 1) * (can_widen(s, rows) ? kWideCols / kCols : 2);
+    return (paged_slots(s) * 17 / 12 + 1) * (can_widen(s, rows) ? kWideCols / kCols : 2);
 }
 
 std::size_t paged_attention_scratch(const em_paged_shape& s, std::size_t, std::size_t rows) {
@@ -1287,7 +1288,7 @@ long long paged_items(const em_paged_shape& s, long long n_seqs, long long rows)
         tiles = std::min(tiles, seqs * (kNarrowMost / kCols));
         tiles += cols / kWideCols + std::min(seqs, cols / (kNarrowMost + 1));
     }
-    const int slots = paged_slots();
+    const int slots = paged_slots(s);
     return tiles * s.n_kv_heads + (can_split(s) ? 2 * slots + slots / 8 + 1 : 0);
 }
 
@@ -1312,7 +1313,7 @@ void run_paged_attention(PagedAttnArgs a, const em_paged_shape& s, float* scratc
                          hipStream_t stream) {
     const auto rows = static_cast<std::size_t>(a.p.rows);
     a.wide = can_widen(s, rows);
-    a.slots = paged_slots();
+    a.slots = paged_slots(s);
     // A stage of fp32 takes twice the products and both splits: us at 192 /
     // 512 positions, three chunks of 200 rows of 8 heads of 64 (fp32) 45 / 62,
     // one of 1205 rows of 24 heads of 96 85 / 116; eight of up to 466 rows of 20
