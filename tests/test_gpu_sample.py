@@ -269,6 +269,18 @@ def test_ties_across_workgroups(R, V):
         check(x, u, settings(R, rng, **kw))
 
 
+@pytest.mark.parametrize("V", [5000, 40000])
+def test_more_infinities_than_are_kept(V):
+    """Of tokens of infinite logits top-k keeps the first, which share the weight."""
+    rng = np.random.default_rng(V)
+    x = logits(4, V, rng)
+    for r, n in enumerate((1, 150, 1500, V)):
+        x[r, np.sort(rng.permutation(V)[:n])] = np.inf
+    for u in (0.0, 0.3, 0.77, 0.9999):
+        for kw in (dict(), dict(k=140), dict(k=600), dict(k=1200, p=0.5), dict(p=0.7), dict(mp=0.5)):
+            check(x, np.full(4, u, np.float32), settings(4, rng, **kw))
+
+
 def test_rows_together_or_alone_agree():
     """A row's draw does not depend on how many rows share the call."""
     rng = np.random.default_rng(11)
