@@ -297,8 +297,8 @@ int em_paged_check(const em_paged_shape* s);
 /* Stores the keys and values of `rows` rows at their positions, the first
  * `rotary` dims of each key and query head (a multiple of 8, 0 for none)
  * rotated by them on the way: pair i by the angle position * freq[i] (rotary /
- * 2 floats, device memory; the angle formed in 64 bits, its cosine and sine
- * rounded to fp32 once), pair i being dims (2i, 2i + 1), the model's, or with
+ * 2 finite floats, device memory; the angle formed in 64 bits, its cosine and
+ * sine rounded to fp32 once, for angles of up to 2^50), pair i being dims (2i, 2i + 1), the model's, or with
  * halves != 0 dims (i, i + rotary / 2). Row r's queries (n_heads heads) are at
  * q + r * q_stride, its keys and values (n_kv_heads) at k and v likewise, all
  * fp32, e.g. columns of one qkv product; the rotated queries go to q_out +
@@ -351,9 +351,10 @@ size_t em_sample_scratch_bytes(size_t rows, size_t vocab);
  *   tokens[r]   the lowest i, in index order, with the kept weights up to and
  *               including i above u times their sum
  *   logprobs[r] ln(w_token / that sum); NULL: not wanted.
- * Weights are formed in 64 bits and summed as integers of 2^-42 or finer (for
- * a vocabulary of up to 2^20; 2^-44 for 2^18), so neither order nor timing
- * changes a result. A NaN or -inf logit is never drawn; logits of +inf share
+ * Weights are formed in 64 bits, those below e^-60 of the largest count as 0;
+ * top-p's sums are integers of 2^-42 or finer (for a vocabulary of up to 2^20;
+ * 2^-44 for 2^18), others are added in 64 bits in a fixed order, so timing
+ * never changes a result. A NaN or -inf logit is never drawn; logits of +inf share
  * all the weight; a row with nothing to draw gives -1 and -inf. u below 0 or
  * NaN counts as 0, from 1 as the largest number below it. vocab is at most
  * 2^20; rows of logits are logits_stride floats apart. Scratch as above. */

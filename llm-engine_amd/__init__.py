@@ -521,7 +521,7 @@ def _rows_of(t, what, dtype, rows, width, device):
             shape[0] != rows or shape[1] < width or (width > 1 and stride[1] != 1):
         raise InvalidArgument(EM_EINVAL, f"{what}: expected {rows} {dtype} rows of {width} on "
                                          f"cuda:{device}")
-    return t.data_ptr(), (stride[0] if rows > 1 else max(stride[0], width))
+    return t.data_ptr(), (stride[0] if rows > 1 else width)
 
 
 _CACHE_DTYPES: list = []

@@ -49,21 +49,6 @@ std::string paged_batch_reject(const em_paged_shape& s, const em_paged_batch& b,
 
 namespace {
 
-template <class T>
-struct CacheValue;
-template <>
-struct CacheValue<float> {
-    static __device__ float of(float x) { return x; }
-};
-template <>
-struct CacheValue<_Float16> {
-    static __device__ _Float16 of(float x) { return static_cast<_Float16>(x); }
-};
-template <>
-struct CacheValue<__bf16> {
-    static __device__ __bf16 of(float x) { return static_cast<__bf16>(x); }
-};
-
 struct AppendArgs {
     PagedArgs p;
     const float *q, *k, *v;
@@ -109,8 +94,8 @@ __device__ __forceinline__ void cos_sin(double angle, float& c, float& s) {
 template <class T>
 __device__ __forceinline__ void store4(T* dst, float a, float b, float c, float d) {
     typedef T vec __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<vec*>(dst) = vec{CacheValue<T>::of(a), CacheValue<T>::of(b),
-                                       CacheValue<T>::of(c), CacheValue<T>::of(d)};
+    *reinterpret_cast<vec*>(dst) = vec{static_cast<T>(a), static_cast<T>(b), static_cast<T>(c),
+                                       static_cast<T>(d)};
 }
 
 // Row blockIdx.x. A thread owns one unit of eight head dims (four pairs: two

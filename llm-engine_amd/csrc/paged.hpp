@@ -45,7 +45,8 @@ std::string paged_batch_reject(const em_paged_shape& s, const em_paged_batch& b,
                                std::size_t rows);
 
 // The sequence that row r belongs to: the last s < n_seqs with row_start[s]
-// <= r, or -1 where there is none or row_start[s + 1] <= r. All 64 lanes of
+// <= r, or -1 where there is none or row_start[s + 1] <= r (starts that fall
+// may hide r's, but never give another). All 64 lanes of
 // the wave call it with one r; a round reads 64 starts and keeps the span
 // between two, so 64 sequences take one memory latency and 4096 two.
 __device__ __forceinline__ int row_sequence(const PagedArgs& a, int r) {
@@ -60,7 +61,7 @@ __device__ __forceinline__ int row_sequence(const PagedArgs& a, int r) {
         if (step == 1) break;
         span = min(step, span - (n - 1) * step);
     }
-    return a.row_start[lo + 1] > r ? lo : -1;
+    return a.row_start[lo] <= r && a.row_start[lo + 1] > r ? lo : -1;
 }
 
 // The first element of position t's slot for kv head 0, or -1 where the

@@ -4,8 +4,8 @@
 //
 // A sequence's new rows and the heads that share a kv head are its columns:
 // column c is row c / group, head kv head * group + c % group. A work item is
-// (sequence, kv head, 16 columns, run of positions), so a key or value is read
-// once for 16 columns. Both products are MFMAs whose terms keep fp32's
+// (sequence, kv head, 16 or 128 columns, run of positions), so a key or value is
+// read once for as many columns. Both products are MFMAs whose terms keep fp32's
 // accuracy (see Ops); the softmax runs with one pass over the positions, a
 // running maximum and sum in fp32.
 //
@@ -23,7 +23,6 @@ namespace em {
 namespace {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kCols = 16;       // columns of a narrow item, and of a unit of partials
 constexpr int kWideCols = 128;  // columns of a wide one
@@ -82,11 +81,6 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s) {
     return w;
 }
 
-__device__ __forceinline__ int wave_sum_int(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
-    return v;
-}
 __device__ __forceinline__ int wave_scan_int(int v) {  // inclusive
     const int lane = threadIdx.x % kWave;
 #pragma unroll
@@ -102,10 +96,12 @@ __device__ __forceinline__ int wave_scan_int(int v) {  // inclusive
 // a half lengths, which twice as many even out (64 sequences of 500 to 4000
 // positions 167 / 146 us, 2 of 100000 189 / 195; a cut costs a wide item its
 // queries' terms again, 2048 rows at 8148 717 / 752).
+// No contraction: both kernels have to come to the same plan.
 struct RunLength {
     float narrow, wide;
 };
 __device__ __forceinline__ RunLength run_length(const PagedAttnArgs& a) {
+#pragma clang fp contract(off)
     const int lane = threadIdx.x % kWave;
     float total = 0.0f, tiles = 0.0f;
     for (int s0 = 0; s0 < a.p.n_seqs; s0 += kWave) {
@@ -128,6 +124,7 @@ __device__ __forceinline__ RunLength run_length(const PagedAttnArgs& a) {
 // Runs of a sequence: its positions over a run's length, to the nearest whole
 // number.
 __device__ __forceinline__ int runs_of(const SeqWork& w, const RunLength& run) {
+#pragma clang fp contract(off)
     const float n = static_cast<float>(w.span) / (w.width == kWideCols ? run.wide : run.narrow);
     return max(1, min(1 << 16, static_cast<int>(n + 0.5f)));
 }
@@ -1368,7 +1365,8 @@ int em_paged_attention(const em_paged_shape* s, const em_paged_batch* b, size_t 
     if (!why.empty()) return fail(EM_EINVAL, why);
     if (window < 0 || window > (1 << 30))
         return fail(EM_EINVAL, "paged_attention: a window of 0 to 2^30 positions");
-    if (!std::isfinite(scale)) return fail(EM_EINVAL, "paged_attention: scale is not finite");
+    if (!std::isfinite(scale * 1.4427f))
+        return fail(EM_EINVAL, "paged_attention: scale is not finite, or its product with log2 e");
     if (rows == 0 || b->n_seqs == 0) return EM_OK;
     const size_t need =
         em::paged_attention_scratch(*s, static_cast<size_t>(b->n_seqs), rows);

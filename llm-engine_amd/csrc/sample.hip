@@ -106,7 +106,7 @@ struct Weigh {
     }
     // Weights side by side and without a branch, so that their chains and table
     // reads overlap (256 x 131072 unfiltered: 65 us, an element at a time 71; 64 x
-    // 32000 with top-p 35 and 40). Not for an endless row.
+    // 32000 of mixed settings 35 and 40). Not for an endless row.
     template <int N>
     __device__ __forceinline__ void several(const float (&x)[N], double (&w)[N]) const {
         double t[N], y[N], q[N];

@@ -97,8 +97,9 @@ def test_append_arguments():
 
 
 def test_attention_arguments():
-    for kw, why in ((dict(window=-1), "window"), (dict(window=(1 << 30) + 1), "window"), (dict(scale=float("inf")), "scale"),
-                    (dict(scale=float("nan")), "scale"), (dict(q=None), "null"),
+    for kw, why in ((dict(window=-1), "window"), (dict(window=(1 << 30) + 1), "window"),
+                    (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"),
+                    (dict(scale=3e38), "scale"), (dict(q=None), "null"),
                     (dict(kc=None), "null"), (dict(vc=None), "null"), (dict(out=None), "null"),
                     (dict(qs=500), "strides"), (dict(os_=514), "strides"), (dict(q=P + 4), "aligned"),
                     (dict(kc=P + 8), "aligned"), (dict(out=P + 4), "aligned")):
