@@ -36,6 +36,7 @@ constexpr int kMaxVocab = 1 << 20;
 constexpr int kHeldBins = 2048, kWideBins = 4096;
 constexpr int kList = 512;   // tokens of a bin that are ranked against each other
 constexpr int kShort = 128;  // a list that holds all that may be kept
+constexpr int kMaxSlices = kWave;  // workgroups a row, where several share one: a lane each
 
 struct SampleArgs {
     int rows, vocab, bits;
@@ -230,7 +231,7 @@ struct SampleShared {
     uint32_t list[kList];
     int list_at[kList];
     double roots[2 * kRoots];
-    double part[kSampleWaves], sums[32];
+    double part[kSampleWaves], sums[kMaxSlices];
     u64 part64[kSampleWaves];
     float part_hi[kSampleWaves], part_lo[kSampleWaves];
     uint32_t part_n[kSampleWaves];
@@ -955,7 +956,6 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
 // more than kList) are done by that workgroup alone, as above. Calls without
 // top-k only.
 
-constexpr int kMaxSlices = 32;
 constexpr int kSliceThreads = 256;
 
 struct SliceRow {
@@ -1303,11 +1303,12 @@ int row_chunks(std::size_t vocab) {
 }
 
 // Slices a row takes, 1: the row kernel, which has rows that LDS holds and many
-// of them. us, row kernel / slices, top-p of 0.9: 1 x 32000 38 / 37, 1 x 50000
-// 60 / 38, 32 x 50000 62 / 63, 1 x 100003 106 / 46, 7 x 100003 107 / 51, 32 x
-// 100003 107 / 77, 64 x 100003 107 / 111; no filter: 41 / 21 at 1 x 100003, 25 /
+// of them. us, row kernel / slices, top-p of 0.9: 1 x 32000 35 / 37, 1 x 50000
+// 60 / 33, 32 x 50000 62 / 59, 1 x 100003 106 / 36, 7 x 100003 107 / 43, 32 x
+// 100003 107 / 64, 64 x 100003 107 / 111; no filter: 41 / 17 at 1 x 100003, 25 /
 // 28 at 64 x 50000. Not with a top-k, which leaves the row kernel little to do
-// after its histogram: 39 / 48 at 7 x 100003, 15 / 27 at 1 x 32000.
+// after its histogram: 39 / 48 at 7 x 100003, 15 / 27 at 1 x 32000. Of 2048
+// logits and more: half as many take 40 at 1 x 100003.
 int slices_of(std::size_t rows, std::size_t vocab) {
     if (row_chunks(vocab) <= kHeldChunks || rows > vocab / 2048) return 1;
     return static_cast<int>(std::min<std::size_t>({kMaxSlices, vocab / 2048, 512 / rows}));
