@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "paged.hpp"
+#include "wave.hpp"
 
 namespace em {
 namespace {
@@ -81,15 +82,20 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s) {
     return w;
 }
 
-__device__ __forceinline__ int wave_scan_int(int v) {  // inclusive
-    const int lane = threadIdx.x % kWave;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        const int o = __shfl_up(v, d, kWave);
-        if (lane >= d) v += o;
+// The work of a lane's sequence of 64, kept from one pass over them to the next
+// (all of a batch of up to 64 is then read once).
+struct LaneWork {
+    SeqWork w;
+    int at = -1;
+    __device__ __forceinline__ const SeqWork& of(const PagedAttnArgs& a, int s0) {
+        if (at != s0) {
+            const int s = s0 + static_cast<int>(threadIdx.x) % kWave;
+            w = s < a.p.n_seqs ? seq_work(a, s) : SeqWork{};
+            at = s0;
+        }
+        return w;
     }
-    return v;
-}
+};
 
 // What all columns' positions cost over the slots. Narrow items take half of that where a
 // sequence would be only a few of them: rounding leaves items of up to one and
@@ -100,19 +106,15 @@ __device__ __forceinline__ int wave_scan_int(int v) {  // inclusive
 struct RunLength {
     float narrow, wide;
 };
-__device__ __forceinline__ RunLength run_length(const PagedAttnArgs& a) {
+__device__ __forceinline__ RunLength run_length(const PagedAttnArgs& a, LaneWork& lanes) {
 #pragma clang fp contract(off)
-    const int lane = threadIdx.x % kWave;
     float total = 0.0f, tiles = 0.0f;
     for (int s0 = 0; s0 < a.p.n_seqs; s0 += kWave) {
-        float t = 0.0f, n = 0.0f;
-        if (s0 + lane < a.p.n_seqs) {
-            const SeqWork w = seq_work(a, s0 + lane);
-            n = static_cast<float>(w.tiles);
-            t = n * static_cast<float>(w.span) * (w.width == kWideCols ? a.wide_cost : 1.0f);
-        }
-        total += wave_sum(t);
-        tiles += wave_sum(n);
+        const SeqWork& w = lanes.of(a, s0);
+        const float n = static_cast<float>(w.tiles);
+        const float t = n * static_cast<float>(w.span) * (w.width == kWideCols ? a.wide_cost : 1.0f);
+        total += last_lane(wave_scan(t));
+        tiles += last_lane(wave_scan(n));
     }
     const float kv = static_cast<float>(a.p.n_kv_heads), slots = static_cast<float>(a.slots);
     const float run = total * kv / slots;
@@ -139,44 +141,41 @@ struct Found {
 };
 // By wave: the sequence for which hit(s, items before, items of it) holds.
 template <class Hit>
-__device__ __forceinline__ bool find(const PagedAttnArgs& a, const RunLength& run, Hit hit, Found& f) {
+__device__ __forceinline__ bool find(const PagedAttnArgs& a, LaneWork& lanes, const RunLength& run,
+                                     Hit hit, Found& f) {
     const int lane = threadIdx.x % kWave;
     int items = 0, units = 0;
     for (int width = a.wide ? kWideCols : kCols; width; width = width == kWideCols ? kCols : 0) {
         for (int s0 = 0; s0 < a.p.n_seqs; s0 += kWave) {
-            const int s = s0 + lane;
-            SeqWork w{};
-            int cells = 0, runs = 0;
-            if (s < a.p.n_seqs) {
-                w = seq_work(a, s);
-                if (w.width == width) cells = w.tiles * a.p.n_kv_heads;
-                runs = runs_of(w, run);
-            }
+            const SeqWork& w = lanes.of(a, s0);
+            const int cells = w.width == width ? w.tiles * a.p.n_kv_heads : 0;
+            int runs = runs_of(w, run);
             // Units by the runs wanted; a sequence that would pass the partials'
             // memory stays whole (its units stay counted: all after it do too).
             const int want = runs > 1 ? cells * runs * (width / kCols) : 0;
-            const int ahead = units + wave_scan_int(want) - want;
+            const int ahead = units + wave_scan(want) - want;
             if (ahead + want > a.part_units) runs = min(runs, 1);
             const int mine = cells * runs;
-            const int before = items + wave_scan_int(mine) - mine;
-            const unsigned long long got = __ballot(mine > 0 && hit(s, before, mine));
+            const int before = items + wave_scan(mine) - mine;
+            const unsigned long long got = __ballot(mine > 0 && hit(s0 + lane, before, mine));
             if (got) {
                 const int src = __ffsll(got) - 1;
+                auto its = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
                 f.seq = s0 + src;
-                f.runs = __shfl(runs, src, kWave);
-                f.item0 = __shfl(before, src, kWave);
-                f.unit0 = __shfl(ahead, src, kWave);
-                f.w.row0 = __shfl(w.row0, src, kWave);
-                f.w.n = __shfl(w.n, src, kWave);
-                f.w.p0 = __shfl(w.p0, src, kWave);
-                f.w.first = __shfl(w.first, src, kWave);
-                f.w.end = __shfl(w.end, src, kWave);
+                f.runs = its(runs);
+                f.item0 = its(before);
+                f.unit0 = its(ahead);
+                f.w.row0 = its(w.row0);
+                f.w.n = its(w.n);
+                f.w.p0 = its(w.p0);
+                f.w.first = its(w.first);
+                f.w.end = its(w.end);
                 f.w.width = width;
-                f.w.tiles = __shfl(w.tiles, src, kWave);
+                f.w.tiles = its(w.tiles);
                 return true;
             }
-            items = __shfl(before + mine, kWave - 1, kWave);
-            units = __shfl(ahead + want, kWave - 1, kWave);
+            items = last_lane(before + mine);
+            units = last_lane(ahead + want);
         }
     }
     return false;
@@ -1120,16 +1119,24 @@ __device__ __forceinline__ void wide_item(const PagedAttnArgs& a, const Item& it
     }
 }
 
+// Workgroups on a CU, four waves each: heads past 128 take a CU's registers.
+// As many as the plan counts on: with a third one of narrow items of heads of 64
+// beside the two, 15 rows of 8 heads at 12921 to 25843 positions (bf16) took 145
+// us for 126.
+constexpr int on_a_cu(int head_size) { return head_size <= 128 ? 2 : 1; }
+
 // WIDE: for calls in which a sequence may have more than kNarrowMost columns.
 template <class T, int DP, bool WIDE>
-__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attn_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(
+    on_a_cu(DP), on_a_cu(DP)))) void paged_attn_kernel(PagedAttnArgs a) {
     constexpr int kNarrowLds = Few<T, DP>::kLds, kWideLds = Wide<T, DP>::kLds;
     __shared__ __attribute__((aligned(16))) char smem[WIDE && kWideLds > kNarrowLds ? kWideLds : kNarrowLds];
     const PagedArgs& p = a.p;
     const int item = blockIdx.x;
     Item it;
-    const RunLength run = run_length(a);
-    if (!find(a, run, [&](int, int before, int mine) { return item >= before && item < before + mine; },
+    LaneWork lanes;
+    const RunLength run = run_length(a, lanes);
+    if (!find(a, lanes, run, [&](int, int before, int mine) { return item >= before && item < before + mine; },
               it.f))
         return;
     // Item order in a sequence: kv heads fastest (the XCDs take blocks in
@@ -1166,7 +1173,8 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, i
     __shared__ __attribute__((aligned(16))) float o_s[kThreads][4];
     __shared__ float2 ml_s[kThreads];
     const int kvh = blockIdx.y, D = p.head_size, tid = threadIdx.x;
-    const RunLength run = run_length(a);
+    LaneWork lanes;
+    const RunLength run = run_length(a, lanes);
     const int last = min(p.rows, (static_cast<int>(blockIdx.x) + 1) * each);
     const int units = p.group * (D / 4), width = min(units, kThreads);
     for (int r = blockIdx.x * each; r < last;) {
@@ -1176,7 +1184,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, i
             continue;
         }
         Found f;
-        if (!find(a, run, [&](int s, int, int) { return s == seq; }, f)) return;
+        if (!find(a, lanes, run, [&](int s, int, int) { return s == seq; }, f)) return;
         const int stop = min(last, f.w.row0 + f.w.n);
         if (f.runs <= 1) {
             r = stop;
@@ -1245,8 +1253,8 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, i
 
 // --- launch ---------------------------------------------------------------------------
 
-// Workgroups the card holds at once: heads past 128 take a CU's registers.
-int paged_slots(const em_paged_shape& s) { return (s.head_size <= 128 ? 2 : 1) * cu_count(); }
+// Workgroups the card holds at once.
+int paged_slots(const em_paged_shape& s) { return on_a_cu(s.head_size) * cu_count(); }
 
 // Whether any sequence of the shape can be split: it needs one and a half
 // runs' positions.
