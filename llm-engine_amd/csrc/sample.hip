@@ -54,7 +54,7 @@ struct SampleArgs {
 };
 
 // A logit as the sampler sees it: NaN is -inf, -0 is 0.
-__device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : -INFINITY; }
+__device__ __forceinline__ float clean(float x) { return fmaxf(x + 0.0f, -INFINITY); }
 // Its bits in an order that is the values'; -inf has the least.
 __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t b = __float_as_uint(x);
@@ -112,7 +112,8 @@ struct Weigh {
     }
     // Weights side by side and without a branch, so that their chains and table
     // reads overlap (256 x 131072 unfiltered: 65 us, an element at a time 71; 64 x
-    // 32000 of mixed settings 35 and 40). Not for an endless row.
+    // 32000 of mixed settings 35 and 40). Not for an endless row; logits below `least`
+    // weigh what it does and are the caller's to leave out.
     template <int N>
     __device__ __forceinline__ void several(const float (&x)[N], double (&w)[N]) const {
         double t[N], y[N], q[N];
@@ -128,8 +129,7 @@ struct Weigh {
         for (int i = 0; i < N; ++i) {
             const int n = static_cast<int>(__double_as_longlong(t[i]));
             q[i] *= small_power(y[i]);
-            const u64 v = __double_as_longlong(q[i]) + (static_cast<u64>(n >> 5) << 52);
-            w[i] = x[i] < least ? 0.0 : __longlong_as_double(v);
+            w[i] = __longlong_as_double(__double_as_longlong(q[i]) + (static_cast<u64>(n >> 5) << 52));
         }
     }
     __device__ __forceinline__ void whole_eight(const float (&x)[8], u64 (&w)[8]) const {
@@ -146,8 +146,7 @@ struct Weigh {
         for (int i = 0; i < 8; ++i) {
             const int n = static_cast<int>(__double_as_longlong(t[i]));
             q[i] *= small_power(z[i]);
-            const u64 v = (__double_as_longlong(q[i]) - (u64{0x3fe} << 52)) >> min(52 - bits - (n >> 5), 63);
-            w[i] = x[i] < least ? 0 : v;
+            w[i] = (__double_as_longlong(q[i]) - (u64{0x3fe} << 52)) >> min(52 - bits - (n >> 5), 63);
         }
     }
     __device__ __forceinline__ double operator()(float x) const {
@@ -555,6 +554,10 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int r, Shared& s
                 const float x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
                 double w[4];
                 weigh.several(x, w);
+                if (__ballot(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])) < weigh.least)) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = x[e] < weigh.least ? 0.0 : w[e];
+                }
                 sum += (w[0] + w[1]) + (w[2] + w[3]);
             }
             most = m;
