@@ -539,6 +539,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int r, Shared& s
     // the maximum, relative to the thread's own so far.
     const bool once = !HELD && !set.greedy && k == 0 && !(top_p < 1.0f) && min_p == 0.0;
     double sum = 0.0;
+    int first = 0;  // greedy: the lowest position of the thread's maximum
     if (once) {
         __syncthreads();  // the roots
         row.batches([&](const float4 (&v)[Row<HELD>::U], int) {
@@ -561,6 +562,11 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int r, Shared& s
                 sum += (w[0] + w[1]) + (w[2] + w[3]);
             }
             most = m;
+        });
+    } else if (set.greedy) {
+        row.template each<true>([&](float x, int pos) {
+            first = x > most ? pos : first;
+            most = fmaxf(most, x);
         });
     } else {
         row.template each<true>([&](float x, int) { most = fmaxf(most, x); });
@@ -639,11 +645,9 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int r, Shared& s
 
     if (set.greedy) {
         // The lowest index of the maximum.
-        int first = 0x7fffffff;
-        row.each([&](float x, int pos) { first = x == top ? min(first, pos) : first; });
         if (tid == 0) s.keep = 0x7fffffff;
         __syncthreads();
-        if (first < 0x7fffffff) atomicMin(&s.keep, first);
+        if (most == top) atomicMin(&s.keep, first);
         __syncthreads();
         if (tid == 0) {
             a.tokens[r] = s.keep - row.pre;
