@@ -296,6 +296,25 @@ def test_many_sequences():
     check_append(Batch(em, 4, 1, 32, 4, seqs, "f16", seed=25), freq(16), True)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_many_long_and_short_sequences(dtype):
+    """The plan over several rounds of 64 sequences: split ones of one row,
+    chunks of many columns and empty ones among short ones."""
+    seqs = [((37 * i) % 90, (1, 1, 0, 2, 1, 5, 1)[i % 7]) for i in range(150)]
+    seqs[3], seqs[70], seqs[140], seqs[149] = (4000, 1), (2500, 12), (300, 40), (6000, 1)
+    b = Batch(em, 16, 2, 64, 16, seqs, dtype, seed=43, lead=2, tail=1)
+    check(b)
+    check(b, window=1500)
+
+
+@pytest.mark.parametrize("heads, kv, D", [(150, 1, 64), (260, 2, 24), (129, 1, 128)])
+def test_more_heads_of_a_kv_head_than_a_tile(heads, kv, D):
+    for dtype in ("f32", "f16", "bf16"):
+        b = Batch(em, heads, kv, D, 16, [(0, 1), (333, 1), (97, 3), (700, 2)], dtype, seed=D)
+        check(b)
+        check(b, window=50)
+
+
 def test_empty_batches():
     b = Batch(em, 4, 1, 32, 4, [(5, 0), (0, 0)], "f32", seed=26, tail=3)
     b.cuda()
