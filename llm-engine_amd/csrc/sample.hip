@@ -18,11 +18,11 @@
 //
 // One workgroup a row, 16 waves each with its own run of consecutive logits;
 // rows of up to 32765 are read once, into LDS, longer ones once a pass (greedy and
-// unfiltered ones once in all). Not bound
-// by the logits' bytes but by the passes of a workgroup one behind the other: 1 x
-// 32000 with top-k of 40 15 us, with top-p of 0.9 34 (four passes over LDS, the
-// 64-bit weights in two of them); 256 x 131072 unfiltered 47 us (its weights 36),
-// with min-p 60 to 70, greedy 27, where a copy's rate would take 26.
+// unfiltered ones once in all). Not bound by the logits' bytes but by the passes
+// of a workgroup one behind the other: 1 x 32000 with top-k of 40 15 us, with
+// top-p of 0.9 34 (four passes over LDS, the 64-bit weights in two of them); 256 x
+// 131072 unfiltered 47 us (its weights 36), with min-p 60 to 70, greedy 27, where
+// a copy's rate would take 26.
 #include <algorithm>
 #include <cmath>
 
