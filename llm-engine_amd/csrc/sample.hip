@@ -201,7 +201,7 @@ struct SampleShared {
     uint32_t part_n[kSampleWaves];
     uint32_t n, key, ties, bin, bin_end;
     u64 left;
-    int token, last, keep;
+    int token, last, keep;  // token, last: the drawing threads (draw_in_run)
 };
 
 // Chunks a wave whose row LDS (160 KB) holds beside SampleShared.
@@ -228,6 +228,22 @@ __device__ __forceinline__ T block_prefix(T v, T* part, T& total) {
         total += p;
     }
     return before + in - v;
+}
+
+// Running sums of v over the workgroup's threads: a thread's own, and `before`
+// its predecessor's, the same bits (own less v would lose what is 2^-53 of v).
+__device__ __forceinline__ double block_running(double v, double* part, double& before) {
+    const double in = wave_scan(v);
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    __syncthreads();
+    if (lane == kWave - 1) part[wave] = in;
+    __syncthreads();
+    double base = 0.0;
+#pragma unroll
+    for (int i = 0; i < kSampleWaves; ++i) base += i < wave ? part[i] : 0.0;
+    const double ahead = __shfl_up(in, 1, kWave);
+    before = lane ? base + ahead : base;
+    return base + in;
 }
 
 // A row's logits, cleaned. HELD: kept in LDS, read from memory once.
@@ -357,7 +373,8 @@ __device__ __forceinline__ int pick_run(double sum, double draw, double& total, 
     target = draw * total;
     const u64 some = __ballot(sum > 0.0), past = __ballot(sum > 0.0 && run > target);
     const int pick = past ? __ffsll(past) - 1 : 63 - __clzll(some);
-    target = fmax(0.0, target - __shfl(run - sum, pick, kWave));
+    const double ahead = __shfl_up(run, 1, kWave);  // the run before's
+    target = fmax(0.0, target - (pick ? __shfl(ahead, pick, kWave) : 0.0));
     return pick;
 }
 
@@ -385,15 +402,20 @@ __device__ __forceinline__ void draw_in_run(const SampleArgs& a, int r, Shared& 
         here = left > n_before ? min(left - n_before, n) : 0;
         mine += here * wt;
     }
-    double all = 0.0;
-    const double before = block_prefix(mine, s.part, all);
-    const bool hit = mine > 0.0 && before <= target && before + mine > target;
-    if (hit) s.token = 1;
-    if (mine > 0.0) atomicMax(&s.last, tid);
+    double before = 0.0;
+    const double through = block_running(mine, s.part, before);
+    // One thread draws: the first with any weight whose running sum passes the
+    // target, the last with any where rounding leaves none. Running sums of equal
+    // real value may round apart (a scan adds in another order for each lane), so
+    // several may pass or none; the lowest index is the same on every call. At a
+    // target of 0 it is the first thread with any weight, however small beside
+    // what follows.
+    const int lane = tid % kWave;
+    const u64 some = __ballot(mine > 0.0), past = __ballot(mine > 0.0 && through > target);
+    if (past && lane == __ffsll(past) - 1) atomicMin(&s.token, tid);
+    if (some && lane == 63 - __clzll(some)) atomicMax(&s.last, tid);
     __syncthreads();
-    // The scan's rounding may leave a gap that the target falls into: the
-    // last thread with any weight then takes it.
-    if (!(hit || (s.token < 0 && tid == s.last))) return;
+    if (tid != (s.token < kSampleThreads ? s.token : s.last)) return;
     double run = before, w_token = 0.0;
     int token = -1;
     for (int p = from; p < to; ++p) {
@@ -583,7 +605,8 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, int r, Shared& s
     }
     if (tid == 0) {
         s.n = 0;
-        s.token = s.last = -1;
+        s.token = kSampleThreads;
+        s.last = -1;
     }
     __syncthreads();
 #pragma unroll
@@ -1212,7 +1235,10 @@ __global__ __launch_bounds__(kSampleThreads) void slice_draw_kernel(SliceArgs b)
         return;
     }
     if (tid < 2 * kRoots) s.roots[tid] = kRoot[tid];
-    if (tid == 0) s.token = s.last = -1;
+    if (tid == 0) {
+        s.token = kSampleThreads;
+        s.last = -1;
+    }
     if (static_cast<uint32_t>(tid) < n) {
         s.list[tid] = row.list[tid];
         s.list_at[tid] = row.list_at[tid];

@@ -1,0 +1,99 @@
+"""Sampling where u leaves one right answer: at 0 (and below, and NaN) the first
+token kept, whatever stands behind it. No rounding decides that, so no other
+token counts. A kept token's weight, relative to the row's largest, is at least
+e^-60. A log-probability is ln(w / sum) rounded to fp32 once (2^-24 of it) from
+weights of 2^-50 and a sum of at most 2^20 of them, far inside 2^-20."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tests import engine
+
+em = engine.load()
+pytestmark = pytest.mark.gpu
+
+# (rows, vocabulary): one workgroup a row with the row in LDS and without, and a
+# row over several workgroups.
+SPREADS = [(3, 3000), (2, 32000), (300, 40000), (1, 50001), (5, 100003)]
+
+
+def weights(x, T):
+    with np.errstate(all="ignore"):
+        z = (x.astype(np.float64) - float(x.max())) / float(np.float32(T))
+        return np.where(z >= -60, np.exp(z), 0.0)
+
+
+def two_or_three(R, V, rng):
+    """Rows of a few tokens 38 to 55 apart, the lightest first: within a wave's
+    run of a row (another thread's, the next lane's, the same thread's) and far
+    behind it; and a whole row far below one token."""
+    x = np.full((R, V), -np.inf, np.float32)
+    heavy = [1, 2, 40, 1500, V - 1, V // 2 + 3]
+    for r in range(R):
+        at = heavy[r % len(heavy)]
+        x[r, 0], x[r, at] = 0.0, 38.0 + 17.0 * rng.random()
+        if r % 3 == 1:
+            x[r, at + 1 if at + 1 < V else at - 1] = x[r, at] + 1.0
+    whole = rng.normal(0, 0.5, V).astype(np.float32)
+    x[R - 1] = whole
+    x[R - 1, min(777, V - 1)] = 45.0
+    return x
+
+
+def draw(x, u, T=1.0, **kw):
+    R = x.shape[0]
+    one = lambda v, t=torch.float32: torch.full((R,), v, dtype=t, device="cuda")
+    kw = {k: one(v, torch.int32 if k == "top_k" else torch.float32) for k, v in kw.items()}
+    tok, lp = em.sample(torch.from_numpy(x).cuda(), one(u), temperature=one(T), **kw)
+    return tok.cpu().numpy(), lp.cpu().numpy()
+
+
+def check(x, tok, lp, w, want, r):
+    assert tok[r] == want, (r, tok[r], want)
+    l = math.log(w[want] / w.sum())
+    assert abs(lp[r] - l) <= 2.0 ** -24 * abs(l) + 2.0 ** -20, (r, lp[r], l)
+
+
+@pytest.mark.parametrize("u", [0.0, -1.0, math.nan])
+@pytest.mark.parametrize("R, V", SPREADS)
+def test_the_first_token_kept(R, V, u):
+    x = two_or_three(R, V, np.random.default_rng(R + V))
+    for T, kw in ((1.0, {}), (1.0, dict(min_p=0.0)), (0.9, dict(top_p=1.0)), (1.0, dict(top_k=0))):
+        tok, lp = draw(x, u, T, **kw)
+        for r in range(R):
+            w = weights(x[r], T)
+            check(x, tok, lp, w, int(np.flatnonzero(w)[0]), r)
+
+
+@pytest.mark.parametrize("R, V", SPREADS)
+def test_the_first_token_of_a_long_top_k(R, V):
+    """More tokens kept than the short list holds."""
+    x = two_or_three(R, V, np.random.default_rng(R * V))
+    k = 200
+    light = 1 + np.arange(k)  # behind the first, as light or lighter
+    x[:, light] = np.where(x[:, light] == -np.inf, -1.0, x[:, light]).astype(np.float32)
+    tok, lp = draw(x, 0.0, top_k=k)
+    for r in range(R):
+        order = np.lexsort((np.arange(V), -x[r]))[:k]
+        w = np.zeros(V)
+        w[order] = weights(x[r], 1.0)[order]
+        check(x, tok, lp, w, int(np.flatnonzero(w)[0]), r)
+
+
+@pytest.mark.parametrize("T", [0.3, 1.0])
+@pytest.mark.parametrize("V", [32000, 50001])
+def test_the_first_token_before_a_far_likelier_one(V, T):
+    rng = np.random.default_rng(V)
+    x = rng.normal(0, 2, (16, V)).astype(np.float32)
+    for r in range(16):
+        x[r, rng.integers(1, 1900)] += np.float32(45.0 * T)
+    tok, lp = draw(x, 0.0, T)
+    for r in range(16):
+        w = weights(x[r], T)
+        z = (x[r].astype(np.float64) - float(x[r].max())) / float(np.float32(T))
+        first = int(np.flatnonzero(w)[0])
+        # No token before it stands at the border of what counts.
+        assert (np.abs(z[:first + 1] + 60) > 1e-3).all()
+        check(x, tok, lp, w, first, r)
