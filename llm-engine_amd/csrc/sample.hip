@@ -1119,15 +1119,15 @@ __global__ __launch_bounds__(kSliceThreads) void slice_count_kernel(SliceArgs b)
 }
 
 // The bin at which top-p ends, from the row's histogram, by a
-// workgroup of THREADS.
+// workgroup of THREADS; part: two sums a wave.
 struct Border {
     int bin;
     uint32_t count;  // tokens up to and with the bin
     u64 left;        // what is wanted of the bin's weight
 };
 template <int THREADS>
-__device__ __forceinline__ Border border_of(const SliceRow& row, const Settings& set, u64* part,
-                                            Border* out) {
+__device__ __forceinline__ Border border_of(const SliceRow& row, const Settings& set,
+                                            u64 (&part)[2 * THREADS / kWave], Border* out) {
     constexpr int E = kWideBins / THREADS;
     const int tid = threadIdx.x, wave = tid / kWave;
     u64 w[E], sum = 0;
@@ -1208,6 +1208,7 @@ __global__ __launch_bounds__(kSliceThreads) void slice_list_kernel(SliceArgs b) 
 
 __global__ __launch_bounds__(kSampleThreads) void slice_draw_kernel(SliceArgs b) {
     __shared__ SampleShared<kWideBins> s;
+    __shared__ u64 part64[2 * kSampleWaves];
     __shared__ Border border;
     const SampleArgs& a = b.a;
     const int r = blockIdx.x, tid = threadIdx.x;
@@ -1225,7 +1226,7 @@ __global__ __launch_bounds__(kSampleThreads) void slice_draw_kernel(SliceArgs b)
     Border end_at{};
     uint32_t n = 0;
     if (view.kind == kTopP) {
-        end_at = border_of<kSampleThreads>(row, set, s.part64, &border);
+        end_at = border_of<kSampleThreads>(row, set, part64, &border);
         n = row.n;
         alone = n > kList;
     }

@@ -1,4 +1,6 @@
-"""Sampling where u leaves one right answer: at 0 (and below, and NaN) the first
+"""Sampling at the ends of its ranges.
+
+Where u leaves one right answer: at 0 (and below, and NaN) the first
 token kept, whatever stands behind it. No rounding decides that, so no other
 token counts. A kept token's weight, relative to the row's largest, is at least
 e^-60. A log-probability is ln(w / sum) rounded to fp32 once (2^-24 of it) from
@@ -10,6 +12,8 @@ import pytest
 import torch
 
 from tests import engine
+from tests.test_gpu_sample import check as check_filters
+from tests.test_gpu_sample import settings
 
 em = engine.load()
 pytestmark = pytest.mark.gpu
@@ -97,3 +101,19 @@ def test_the_first_token_before_a_far_likelier_one(V, T):
         # No token before it stands at the border of what counts.
         assert (np.abs(z[:first + 1] + 60) > 1e-3).all()
         check(x, tok, lp, w, first, r)
+
+
+@pytest.mark.parametrize("R, V", [(2, 50001), (9, 100003)])
+@pytest.mark.parametrize("part", range(16))
+def test_top_p_ends_in_every_part_of_the_weights(part, R, V):
+    """One token of weight 1 and the rest around 2^-(2 part + 1) of it, half of
+    whose weight top-p keeps: the border lies in each sixteenth of the 2^-32
+    that the histogram of a row over several workgroups covers."""
+    rng = np.random.default_rng(part + V)
+    x = (-math.log(2) * (2 * part + 2 * rng.random((R, V)))).astype(np.float32)
+    at = rng.integers(0, V, R)
+    x[np.arange(R), at] = 0.5
+    rest = np.exp(x.astype(np.float64) - 0.5).sum(1) - 1
+    p = ((1 + rest / 2) / (1 + rest)).astype(np.float32)
+    for u in (0.0, 0.37, 0.999):
+        check_filters(x, np.full(R, u, np.float32), settings(R, rng, p=p))
