@@ -171,10 +171,7 @@ struct Weigh {
     }
 };
 
-// A share in [0, 1) of a sum of weights, exactly: rounded down, and up.
-__device__ __forceinline__ u64 share_down(u64 total, float share) {
-    return __umul64hi(total, static_cast<u64>(static_cast<double>(share) * 0x1p64));
-}
+// A share in [0, 1) of a sum of weights, exactly and rounded up.
 __device__ __forceinline__ u64 share_up(u64 total, float share) {
     const u64 f = static_cast<u64>(static_cast<double>(share) * 0x1p64);
     return __umul64hi(total, f) + (total * f != 0);
@@ -437,15 +434,18 @@ __device__ __forceinline__ void draw_in_run(const SampleArgs& a, int r, Shared& 
     if (a.logprobs) a.logprobs[r] = static_cast<float>(log(w_token / total));
 }
 
-// Draws from the n tokens of the list (keys and positions), all that may be
-// kept among them: ranks them, keeps the highest most_kept, of those what top-p
-// (nucleus) and min-p leave, which are some of the highest ranks too.
+// Draws from the n tokens of the list (keys and positions, at most kShort), all
+// that may be kept among them: ranks them, keeps the highest most_kept, of those what top-p
+// (nucleus, by whole weights) and min-p leave, which are some of the highest
+// ranks too.
 template <class Shared>
 __device__ __forceinline__ void draw_from_list(const SampleArgs& a, int r, Shared& s,
                                                const Settings& set, const Weigh& weigh, uint32_t n,
                                                uint32_t most_kept, bool nucleus) {
     const int tid = threadIdx.x;
-    uint32_t key = 0, rank = 0;
+    auto* weights = reinterpret_cast<double*>(s.weight + kShort);
+    static_assert(kShort == 2 * kWave && Shared::kBins >= 2 * kShort);
+    uint32_t key = 0, rank = 0, place = 0;  // place: rank by position
     int pos = 0;
     const bool mine = static_cast<uint32_t>(tid) < n;
     if (mine) {
@@ -456,51 +456,44 @@ __device__ __forceinline__ void draw_from_list(const SampleArgs& a, int r, Share
             const uint32_t o = s.list[i];
             const int at = s.list_at[i];
             rank += (o > key) | ((o == key) & (at < pos));
+            place += at < pos;
         }
     }
-    n = min(n, most_kept);
-    const bool in = mine && rank < n;
+    most_kept = min(n, most_kept);
+    const bool in = mine && rank < most_kept;
     const float x = key_value(key);
     const double w = in ? weigh(x) : 0.0;
     const u64 ww = in ? weigh.whole(x) : 0;
-    if (tid == 0) s.keep = n;
+    if (tid == 0) s.keep = most_kept;
     __syncthreads();  // the list has been read
-    if (in) {
-        s.weight[rank] = ww;
-        s.list_at[rank] = pos;
-    }
+    if (in) s.weight[rank] = ww;
+    if (mine) s.list_at[place] = pos;
     __syncthreads();
-    if (in) {
+    if (in && nucleus) {
         u64 before = 0, total = 0;
 #pragma unroll 8
-        for (uint32_t i = 0; i < n; ++i) {
+        for (uint32_t i = 0; i < most_kept; ++i) {
             const u64 o = s.weight[i];
             before += i < rank ? o : 0;
             total += o;
         }
-        if (nucleus) {
-            const u64 target = max(u64{1}, share_up(total, fmaxf(set.top_p, 0.0f)));
-            if (rank > 0 && before >= target) atomicMin(&s.keep, static_cast<int>(rank));
-        }
-        if (w < set.min_p) atomicMin(&s.keep, static_cast<int>(rank));
+        const u64 target = max(u64{1}, share_up(total, fmaxf(set.top_p, 0.0f)));
+        if (rank > 0 && before >= target) atomicMin(&s.keep, static_cast<int>(rank));
     }
+    if (in && w < set.min_p) atomicMin(&s.keep, static_cast<int>(rank));
     __syncthreads();
-    const uint32_t keep = s.keep;
-    if (!in || rank >= keep) return;
-    u64 before = 0, total = 0;
-#pragma unroll 8
-    for (uint32_t i = 0; i < keep; ++i) {
-        const u64 o = s.weight[i];
-        const int at = s.list_at[i];
-        before += at < pos ? o : 0;
-        total += o;
-    }
-    const u64 target = set.draw < 1.0 ? share_down(total, static_cast<float>(set.draw)) : total - 1;
-    if (before <= target && before + ww > target) {
-        a.tokens[r] = pos;
-        if (a.logprobs)
-            a.logprobs[r] = static_cast<float>(log(ldexp(w, a.bits) / static_cast<double>(total)));
-    }
+    // The draw: weights in 64 bits (whole ones would leave nothing of those below
+    // 2^-bits) in the order of positions, two a lane of one wave.
+    if (mine) weights[place] = rank < static_cast<uint32_t>(s.keep) ? w : 0.0;
+    __syncthreads();
+    if (tid >= kWave) return;
+    const uint32_t at = 2 * tid;
+    const double w0 = at < n ? weights[at] : 0.0, w1 = at + 1 < n ? weights[at + 1] : 0.0;
+    double total = 0.0, target = 0.0;
+    if (tid != pick_run(w0 + w1, set.draw, total, target)) return;
+    const bool second = w1 > 0.0 && !(w0 > target);
+    a.tokens[r] = s.list_at[at + second];
+    if (a.logprobs) a.logprobs[r] = static_cast<float>(log((second ? w1 : w0) / total));
 }
 
 // The last token that top-p keeps, from the list's tokens of the border bin

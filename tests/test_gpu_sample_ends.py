@@ -86,6 +86,22 @@ def test_the_first_token_of_a_long_top_k(R, V):
         check(x, tok, lp, w, int(np.flatnonzero(w)[0]), r)
 
 
+@pytest.mark.parametrize("k", [2, 3, 40, 128])
+@pytest.mark.parametrize("R, V", SPREADS + [(1, 1 << 20)])
+def test_the_first_token_of_a_short_top_k(R, V, k):
+    """Tokens kept of 2^-55 to 2^-81 of the largest have a weight too."""
+    x = two_or_three(R, V, np.random.default_rng(R * V + k))
+    if R == 1:
+        x[0] = np.where(np.arange(V) == V // 3, 0.0, np.where(np.arange(V) == V - 9, 41.0, -30.0))
+    for u in (0.0, 2.0 ** -90):  # below every share but the first's
+        tok, lp = draw(x, u, top_k=k)
+        for r in range(R):
+            order = np.lexsort((np.arange(V), -x[r]))[:k]
+            w = np.zeros(V)
+            w[order] = weights(x[r], 1.0)[order]
+            check(x, tok, lp, w, int(np.flatnonzero(w)[0]), r)
+
+
 @pytest.mark.parametrize("T", [0.3, 1.0])
 @pytest.mark.parametrize("V", [32000, 50001])
 def test_the_first_token_before_a_far_likelier_one(V, T):
