@@ -356,8 +356,8 @@ size_t em_sample_scratch_bytes(size_t rows, size_t vocab);
  * 2^-44 for 2^18), others are added in 64 bits in a fixed order, so timing
  * never changes a result. A NaN or -inf logit is never drawn; logits of +inf share
  * all the weight; a row with nothing to draw gives -1 and -inf. u below 0 or
- * NaN counts as 0, from 1 as the largest number below it. vocab is at most
- * 2^20; rows of logits are logits_stride floats apart. Scratch as above. */
+ * NaN counts as 0, from 1 as 1 - 2^-53, the largest 64-bit number below it.
+ * vocab is at most 2^20; rows of logits are logits_stride floats apart. Scratch as above. */
 int em_sample(size_t rows, size_t vocab, const float* logits, size_t logits_stride, const float* u,
               const em_sampling* settings, int* tokens, float* logprobs, void* scratch,
               void* stream);

@@ -332,7 +332,7 @@ struct Settings {
         top_p = a.top_p ? a.top_p[r] : 1.0f;
         const float mp = a.min_p ? a.min_p[r] : 0.0f, u = a.u[r];
         min_p = mp > 0.0f ? fmin(static_cast<double>(mp), 1.0) : 0.0;
-        draw = u > 0.0f ? fmin(static_cast<double>(u), 1.0) : 0.0;
+        draw = u > 0.0f ? fmin(static_cast<double>(u), 0x1.fffffffffffffp-1) : 0.0;
     }
 };
 

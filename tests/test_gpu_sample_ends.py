@@ -133,3 +133,21 @@ def test_top_p_ends_in_every_part_of_the_weights(part, R, V):
     p = ((1 + rest / 2) / (1 + rest)).astype(np.float32)
     for u in (0.0, 0.37, 0.999):
         check_filters(x, np.full(R, u, np.float32), settings(R, rng, p=p))
+
+
+@pytest.mark.parametrize("u", [1.0, 2.0, math.inf])
+@pytest.mark.parametrize("kw", [{}, dict(top_k=2), dict(top_k=200), dict(min_p=1e-30)], ids=str)
+@pytest.mark.parametrize("R, V", SPREADS)
+def test_u_from_one_is_one_less_2_to_minus_53(R, V, kw, u):
+    """A last token of e^-30 of the sum (2^-43) is drawn by it, one of e^-40
+    (2^-58) not: both far from the border."""
+    x = np.full((R, V), -np.inf, np.float32)
+    heavy = (np.arange(R) * 37) % (V - 1)
+    far = np.where(np.arange(R) % 2 == 0, 30.0, 40.0)
+    behind = np.minimum(heavy + 1 + (np.arange(R) * 997) % V, V - 1)
+    x[np.arange(R), heavy] = 5.0
+    x[np.arange(R), behind] = (5.0 - far).astype(np.float32)
+    tok, lp = draw(x, u, **kw)
+    for r in range(R):
+        want = int(behind[r] if far[r] == 30.0 else heavy[r])
+        check(x, tok, lp, weights(x[r], 1.0), want, r)
