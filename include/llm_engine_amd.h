@@ -259,8 +259,9 @@ int em_attention(const em_attention_shape* s, size_t rows, const int* pos_dev, c
  * row r is at position lengths[s] - (row_start[s + 1] - r), lengths[s] counting
  * the batch's own rows. Position t of the sequence is slot t % page_size of
  * page page_table[s * table_stride + t / page_size]. row_start must not fall;
- * a sequence may have no rows. Rows outside [row_start[0], row_start[n_seqs])
- * (a padded batch) are nobody's: no operator writes anything for them.
+ * a sequence may have no rows, and one whose rows are not all the call's
+ * (row_start[s] < 0 or row_start[s + 1] past its row count) has none. Rows of no
+ * sequence (a padded batch) are nobody's: no operator writes anything for them.
  * Positions that do not exist (negative ones, those past max_pages *
  * page_size) and pages outside [0, n_pages) hold nothing: nothing is stored
  * there and attention does not see them. No counterpart in the reference,

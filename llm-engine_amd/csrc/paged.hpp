@@ -44,9 +44,15 @@ std::string paged_reject(const em_paged_shape& s);
 std::string paged_batch_reject(const em_paged_shape& s, const em_paged_batch& b,
                                std::size_t rows);
 
+// Whether rows [r0, r1) are a sequence's: all of them the call's. Others' are
+// nobody's, in every operator.
+__device__ __forceinline__ bool rows_exist(const PagedArgs& a, int r0, int r1) {
+    return r0 >= 0 && r1 <= a.rows && r1 > r0;
+}
+
 // The sequence that row r belongs to: the last s < n_seqs with row_start[s]
-// <= r, or -1 where there is none or row_start[s + 1] <= r (starts that fall
-// may hide r's, but never give another). All 64 lanes of
+// <= r, or -1 where there is none or its rows do not exist or end before r
+// (starts that fall may hide r's, but never give another). All 64 lanes of
 // the wave call it with one r; a round reads 64 starts and keeps the span
 // between two, so 64 sequences take one memory latency and 4096 two.
 __device__ __forceinline__ int row_sequence(const PagedArgs& a, int r) {
@@ -61,7 +67,8 @@ __device__ __forceinline__ int row_sequence(const PagedArgs& a, int r) {
         if (step == 1) break;
         span = min(step, span - (n - 1) * step);
     }
-    return a.row_start[lo] <= r && a.row_start[lo + 1] > r ? lo : -1;
+    const int r0 = a.row_start[lo], r1 = a.row_start[lo + 1];
+    return rows_exist(a, r0, r1) && r0 <= r && r1 > r ? lo : -1;
 }
 
 // The first element of position t's slot for kv head 0, or -1 where the

@@ -69,7 +69,7 @@ __device__ __forceinline__ SeqWork seq_work(const PagedAttnArgs& a, int s) {
     SeqWork w;
     w.row0 = p.row_start[s];
     const int r1 = p.row_start[s + 1];
-    w.n = w.row0 >= 0 && r1 <= p.rows && r1 > w.row0 ? r1 - w.row0 : 0;
+    w.n = rows_exist(p, w.row0, r1) ? r1 - w.row0 : 0;
     const int len = max(p.lengths[s], -(1 << 29));
     const int cap = p.page_size * p.max_pages;
     w.p0 = len - w.n;
@@ -1185,12 +1185,11 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(PagedAttnArgs a, i
     const int units = p.group * (D / 4), width = min(units, kThreads);
     for (int r = blockIdx.x * each; r < last;) {
         const int seq = row_sequence(p, r);
-        if (seq < 0) {
+        Found f;
+        if (seq < 0 || !find(a, lanes, run, [&](int s, int, int) { return s == seq; }, f)) {
             ++r;
             continue;
         }
-        Found f;
-        if (!find(a, lanes, run, [&](int s, int, int) { return s == seq; }, f)) return;
         const int stop = min(last, f.w.row0 + f.w.n);
         if (f.runs <= 1) {
             r = stop;
