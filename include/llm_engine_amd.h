@@ -304,8 +304,8 @@ int em_paged_check(const em_paged_shape* s);
  * q + r * q_stride, its keys and values (n_kv_heads) at k and v likewise, all
  * fp32, e.g. columns of one qkv product; the rotated queries go to q_out +
  * r * q_out_stride, which may be q itself. q NULL: keys and values alone.
- * A row at a position that does not exist is left alone; one whose page holds
- * nothing has its queries rotated. Two rows at one slot leave either's values.
+ * A row at a position that does not exist is left alone, q_out's too; one whose
+ * page holds nothing has its queries rotated. Two rows at one slot leave either's values.
  * Pointers 16-byte aligned, row strides multiples of 4. */
 int em_paged_append(const em_paged_shape* s, const em_paged_batch* b, size_t rows, const float* q,
                     size_t q_stride, const float* k, size_t k_stride, const float* v,
@@ -321,7 +321,9 @@ size_t em_paged_attention_scratch_floats(const em_paged_shape* s, size_t n_seqs,
  * positions t <= p, with window > 0 those past p - window alone, of kv head
  * h / (n_heads / n_kv_heads): out = sum_t softmax_t(scale * q . k_t) v_t. scale
  * 0 is 1 / sqrt(head_size). Positions a row does not see never reach its
- * output, whatever their slots hold. A row that sees nothing gets zeros.
+ * output, whatever their slots hold. A row that sees nothing gets zeros. A row
+ * past the table's last position sees the table's, by the query it is given
+ * (append leaves that one alone): lengths[s] belongs within the table.
  * Scratch is the caller's, used by this call alone until it has run; it needs
  * no zero fill. Results are bit-identical across calls of one shape, batch
  * and row count. Pointers 16-byte aligned, row strides multiples of 4. */

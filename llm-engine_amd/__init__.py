@@ -556,7 +556,8 @@ def paged_append(shape: PagedShape, row_start, lengths, page_table, q, k, v, key
     """em_paged_append on torch tensors: q (or None), k and v are 2-D fp32,
     row-strided views allowed; freq holds rotary / 2 floats (None: no
     rotation). Returns the rotated queries: q_out (q itself to rotate in
-    place) or a new tensor."""
+    place) or a new tensor, with zeros in rows that are no sequence's or at
+    positions that do not exist, which a given q_out keeps as they were."""
     import torch
     f32 = torch.float32
     device, s = _here(stream)
@@ -567,7 +568,7 @@ def paged_append(shape: PagedShape, row_start, lengths, page_table, q, k, v, key
     if q is not None:
         qp, qs = _rows_of(q, "q", f32, rows, dim, device)
         if q_out is None:
-            q_out = _new(torch.empty, stream, rows, dim, dtype=f32)
+            q_out = _new(torch.zeros, stream, rows, dim, dtype=f32)
         op, os_ = _rows_of(q_out, "q_out", f32, rows, dim, device)
     kp, ks = _rows_of(k, "k", f32, rows, kv, device)
     vp, vs = _rows_of(v, "v", f32, rows, kv, device)

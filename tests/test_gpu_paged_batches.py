@@ -2,6 +2,7 @@
 starts that leave the call's rows, against the 64-bit definitions of
 paged_ref.py with the tolerances of test_gpu_paged.py."""
 import pytest
+import torch
 
 from tests import engine
 from tests.paged_ref import Batch
@@ -54,3 +55,25 @@ def test_no_row_is_the_calls():
     got = check(b)
     assert (got == -7.0).all()
     check_append(Cut(em, 8, 2, 64, 16, [(0, 0), (2000, 5)], "f32", seed=71, lead=1), freq(32), False)
+
+
+def test_new_queries_hold_zeros_where_nothing_is_rotated():
+    """Rows that are nobody's or at positions that do not exist, in memory that
+    held something else before."""
+    b = Batch(em, 8, 2, 64, 16, [(37, 3), (0, 4), (5, 1)], "bf16", seed=72, lead=2, tail=3,
+              spare_columns=0)
+    b.lengths[1] = 2                     # its first two rows at -2, -1
+    b.lengths[2] = b.max_pages * 16 + 1  # its row past the table
+    f = freq(32)
+    want, _, _ = b.ref_append(f, True)
+    left = torch.isnan(want)
+    assert left.any(1).tolist() == [True] * 2 + [False] * 3 + [True] * 2 + [False] * 2 + [True] * 4
+    b.cuda()
+    for _ in range(8):
+        old = [torch.full((b.rows, 512), float("nan"), device="cuda") for _ in range(4)]
+        del old
+        got = em.paged_append(b.shape, *b.batch(), b.q(), b.k(), b.v(), b.kc, b.vc, freq=f,
+                              halves=True).double().cpu()
+        assert (got[left] == 0).all()
+        top = float(b.qkv.abs().max()) * 2
+        assert ((got - want)[~left].abs() <= 4 * 2.0 ** -24 * top).all()
