@@ -190,8 +190,10 @@ __device__ __forceinline__ bool find(const PagedAttnArgs& a, LaneWork& lanes, co
 //   fp32 caches: both sides three bf16 terms; the three products of the
 //     smallest (below 2^-24 of the whole) are left out: six products.
 //   fp16 caches: two fp16 terms of a column scaled to a largest query value
-//     of 2^14 (weights: 2^14 for 1), off by 2^-22 of the value and 2^-39 of the
-//     largest; fp16 keys and values are at most 2^16: two products.
+//     of 2^14 (weights: 2^14 for 1), off by 2^-22 of the value or, where that is
+//     more, 2^-39 of the largest; fp16 keys and values are at most 2^16: two
+//     products. Of queries the second is held below 2^-20 in a score (small_dims),
+//     of weights it is 2^-39 of a value each.
 template <class T>
 struct Ops;
 
@@ -271,6 +273,29 @@ __device__ __forceinline__ void split_terms(const float (&v)[8], f16x8 (&t)[2], 
         t[1][e] = static_cast<_Float16>(v[e] - static_cast<float>(t[0][e]));
     }
 }
+
+// What two fp16 terms leave of the values past 2^-22 of each: of those so far
+// below a column's largest that their second term is subnormal. bf16's terms say
+// by `lost` what they leave.
+template <class F, int NT>
+__device__ __forceinline__ float small_dims(const float (&)[8], const F (&)[NT]) {
+    return 0.0f;
+}
+__device__ __forceinline__ float small_dims(const float (&v)[8], const f16x8 (&t)[2]) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float left =
+            fabsf(v[e] - static_cast<float>(t[0][e]) - static_cast<float>(t[1][e]));
+        sum += left > 0x1p-22f * fabsf(v[e]) ? left : 0.0f;
+    }
+    return sum;
+}
+// The score that a column's left bits make at most with keys of 65504, in log2
+// units, may be 2^-20 (fp32's rounding of a score of 16); a column that may pass it is
+// done plainly. A query of ordinary size (largest dim times scale log2 e below 2)
+// passes with eight such dims.
+constexpr float kMostLeft = 0x1p-20f / 65504.0f;
 
 // 16-bit caches are loaded as they are (four dwords for eight values), fp32 as
 // two vectors.
@@ -506,7 +531,7 @@ __device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& 
     // The column's query terms.
     typename F::Frag q[kQueryLds ? 1 : C][NT];
     uint32_t lost_q = 0, lost_v = 0;
-    float top_q = 0.0f, unscale = 1.0f;
+    float top_q = 0.0f, unscale = 1.0f, left_q = 0.0f;
     {
         float v[C][8];
         const float* src = a.q + row * a.q_stride + head * D;
@@ -538,6 +563,7 @@ __device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& 
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             split_terms(v[c], q[kQueryLds ? 0 : c], lost_q);
+            left_q += small_dims(v[c], q[kQueryLds ? 0 : c]);
             if (kQueryLds && w == 0) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t) q_s[(c * NT + t) * kWave + lane] = q[0][t];
@@ -550,6 +576,7 @@ __device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& 
     bool bad = KT == 3   ? (lost_q & 0xffffu) != 0 || !(top_q < 0x1p90f)
                : NT == 3 ? (lost_q & 0xffffu) != 0
                          : top_q != 0.0f && !(top_q >= 0x1p-100f && top_q < INFINITY);
+    if constexpr (NT == 2) bad |= sum32(sum16(left_q)) * unscale > kMostLeft;
 
     const T* kc = static_cast<const T*>(a.kc) + kvh * p.head_stride;
     const T* vc = static_cast<const T*>(a.vc) + kvh * p.head_stride;
@@ -844,7 +871,7 @@ __device__ __forceinline__ void wide_item(const PagedAttnArgs& a, const Item& it
 
     Frag q[C][NQ];
     uint32_t lost_q = 0, lost_v = 0;
-    float top_q = 0.0f, unscale = 1.0f;
+    float top_q = 0.0f, unscale = 1.0f, left_q = 0.0f;
     {
         const float* src = a.q + row * a.q_stride + head * D;
         auto load = [&](int c, float (&v)[8]) {
@@ -888,12 +915,14 @@ __device__ __forceinline__ void wide_item(const PagedAttnArgs& a, const Item& it
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] *= up;
                 split_terms(v, q[c], lost_q);
+                left_q += small_dims(v, q[c]);
             }
         }
     }
     bool bad = KT == 3   ? (lost_q & 0xffffu) != 0 || !(top_q < 0x1p90f)
                : NT == 3 ? (lost_q & 0xffffu) != 0
                          : top_q != 0.0f && !(top_q >= 0x1p-100f && top_q < INFINITY);
+    if constexpr (NT == 2) bad |= sum32(left_q) * unscale > kMostLeft;
 
     // Unit x = tid + 256 y of a stage: position x / (DP / 8), head dims 8 (x % (DP / 8)).
     constexpr int UR = DP / 8;

@@ -1,6 +1,8 @@
 """Paged batches that the header defines and other tests do not reach: row
-starts that leave the call's rows, against the 64-bit definitions of
+starts that leave the call's rows, operands of far apart sizes, against the 64-bit definitions of
 paged_ref.py with the tolerances of test_gpu_paged.py."""
+import math
+
 import pytest
 import torch
 
@@ -77,3 +79,51 @@ def test_new_queries_hold_zeros_where_nothing_is_rotated():
         assert (got[left] == 0).all()
         top = float(b.qkv.abs().max()) * 2
         assert ((got - want)[~left].abs() <= 4 * 2.0 ** -24 * top).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads, kv, D", [(4, 2, 64), (8, 1, 128), (3, 3, 80), (2, 1, 256)])
+@pytest.mark.parametrize("small", [-16, -8, -3])
+def test_small_query_dims_beside_a_large_one(dtype, heads, kv, D, small):
+    """The large dims meet keys of zero, the small ones large keys: the scores
+    are made of bits far below the column's largest."""
+    b = Batch(em, heads, kv, D, 16, [(100, 1), (20, 40), (300, 1), (64, 3)], dtype, seed=80 - small)
+    b.q()[:] *= 2.0 ** small
+    b.q()[:, 3::D] = 2.0 ** 13
+    b.kc *= 2.0 ** 13
+    b.view(b.kc)[..., 3] = 0
+    assert b.kc.isfinite().all()
+    check(b)
+
+
+def test_ordinary_queries_with_small_dims():
+    """Dims of 0 and of a millionth of the others beside ordinary ones."""
+    for dtype in ("f16", "bf16"):
+        b = Batch(em, 8, 2, 128, 16, [(500, 1), (20, 40)], dtype, seed=90, q_scale=4.0)
+        b.q()[:, 5::7] *= 1e-6
+        b.q()[:, 6::7] = 0.0
+        check(b)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [1, 20])
+def test_many_small_weights(dtype, rows):
+    """20000 positions of value 1 and weight e^-21 beside one of value 0: sums of
+    equal terms, at most one rounding (2^-24) each, scores of one product (21
+    2^-24 and as much in log2 units), and over fp16 2^-39 a weight."""
+    n = 20000
+    b = Batch(em, 8, 2, 64, 64, [(n, rows)], dtype, seed=91)
+    b.q()[:] = 0.0
+    b.q()[:, ::64] = 1.0
+    kv, vv = b.view(b.kc), b.view(b.vc)
+    kv[:], vv[:] = 0.0, 1.0
+    kv[..., 0] = -21.0
+    p = b.page(0, 0)
+    kv[p, 0], vv[p, 0] = 0.0, 0.0
+    b.cuda()
+    got = em.paged_attention(b.shape, *b.batch(), b.q(), b.kc, b.vc, scale=1.0).double().cpu()
+    for r in range(rows):
+        s = (n + r) * math.exp(-21.0)
+        want = s / (1 + s)
+        tol = want * (n + r + 200) * 2.0 ** -24 + (n + r) * 2.0 ** -39 * (dtype == "f16")
+        assert float((got[r] - want).abs().max()) <= tol
