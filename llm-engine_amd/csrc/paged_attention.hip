@@ -361,7 +361,10 @@ struct __attribute__((aligned(16))) Eight {
 // whose operands the terms do not hold, and for those beside a position that
 // is not finite and that they do not see (its zero weight would not hide it).
 // m, l: maximum (of log2 weights) and sum; o[i]: head dim lane + 64 i,
-// unnormalised.
+// unnormalised. Where a sum passes kLargest they are formed again with m higher by
+// 60: the same weights, l and o 2^60 lower, so that the sums behind a mean of values
+// near fp32's largest are finite, here and when runs are added.
+constexpr float kLargest = 0x1p100f;  // 2^18 runs and waves of it still add up
 template <class T, int N>
 __device__ __forceinline__ void plain_column(const PagedAttnArgs& a, int seq, int row, int head,
                                           int pq, int lo, int hi, int width, int stride, float& m,
@@ -373,53 +376,72 @@ __device__ __forceinline__ void plain_column(const PagedAttnArgs& a, int seq, in
     const long long hoff = (head / p.group) * p.head_stride;
     const T* kc = static_cast<const T*>(a.kc) + hoff;
     const T* vc = static_cast<const T*>(a.vc) + hoff;
-    m = -INFINITY;
-    l = 0.0f;
+    float pre = 1.0f;  // on the weights of o
+    while (true) {
+        m = -INFINITY;
+        l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = 0.0f;
-    for (int t0 = lo; t0 < hi; t0 += stride) {
-        const int t = t0 + lane;
-        uint32_t unit = kNoSlot;
-        if (lane < width && t < hi && t <= pq && !(a.window && t <= pq - a.window))
-            unit = slot_unit(p, seq, t);
-        float x = -INFINITY;
-        if (unit != kNoSlot) {
-            const T* k = kc + static_cast<std::size_t>(unit) * 8;
-            float dot = 0.0f;
-            for (int d = 0; d < D; d += 8) {
-                const auto y = *reinterpret_cast<const Eight<T>*>(k + d);
+        for (int i = 0; i < N; ++i) o[i] = 0.0f;
+        for (int t0 = lo; t0 < hi; t0 += stride) {
+            const int t = t0 + lane;
+            uint32_t unit = kNoSlot;
+            if (lane < width && t < hi && t <= pq && !(a.window && t <= pq - a.window))
+                unit = slot_unit(p, seq, t);
+            float x = -INFINITY;
+            if (unit != kNoSlot) {
+                const T* k = kc + static_cast<std::size_t>(unit) * 8;
+                float dot = 0.0f;
+                for (int d = 0; d < D; d += 8) {
+                    const auto y = *reinterpret_cast<const Eight<T>*>(k + d);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) dot = fmaf(q[d + e], static_cast<float>(y.v[e]), dot);
-            }
-            x = dot * a.scale2;
-        }
-        const float mn = fmaxf(m, wave_max(x));
-        const float alpha = mn == -INFINITY ? 1.0f : exp2f(m - mn);
-        const float w = unit == kNoSlot || x == -INFINITY ? 0.0f : exp2f(x - mn);
-        m = mn;
-        l = l * alpha + wave_sum(w);
-#pragma unroll
-        for (int i = 0; i < N; ++i) o[i] *= alpha;
-        // Eight positions' values in flight; those not seen read slot 0 and count
-        // for nothing, whatever it holds.
-        for (int i = 0; i < width; i += 8) {
-            float v[8][N], wi[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t u = __shfl(unit, i + e, kWave);
-                wi[e] = __shfl(w, i + e, kWave);
-                const T* src = vc + static_cast<std::size_t>(u == kNoSlot ? 0 : u) * 8;
-#pragma unroll
-                for (int n = 0; n < N; ++n) {
-                    const float y = static_cast<float>(src[min(lane + kWave * n, D - 1)]);
-                    v[e][n] = u == kNoSlot ? 0.0f : y;
+                    for (int e = 0; e < 8; ++e) dot = fmaf(q[d + e], static_cast<float>(y.v[e]), dot);
                 }
+                x = dot * a.scale2;
             }
+            const float mn = fmaxf(m, wave_max(x));
+            const float alpha = mn == -INFINITY ? 1.0f : exp2f(m - mn);
+            const float w = unit == kNoSlot || x == -INFINITY ? 0.0f : exp2f(x - mn);
+            m = mn;
+            l = l * alpha + wave_sum(w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int i = 0; i < N; ++i) o[i] *= alpha;
+            // Eight positions' values in flight; those not seen read slot 0 and count
+            // for nothing, whatever it holds.
+            for (int i = 0; i < width; i += 8) {
+                float v[8][N], wi[8];
 #pragma unroll
-                for (int n = 0; n < N; ++n) o[n] = fmaf(wi[e], v[e][n], o[n]);
+                for (int e = 0; e < 8; ++e) {
+                    const uint32_t u = __shfl(unit, i + e, kWave);
+                    wi[e] = __shfl(w * pre, i + e, kWave);
+                    const T* src = vc + static_cast<std::size_t>(u == kNoSlot ? 0 : u) * 8;
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        const float y = static_cast<float>(src[min(lane + kWave * n, D - 1)]);
+                        v[e][n] = u == kNoSlot ? 0.0f : y;
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int n = 0; n < N; ++n) o[n] = fmaf(wi[e], v[e][n], o[n]);
+            }
         }
+        if (std::is_same_v<T, _Float16>) break;  // at most 2^46
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(o[i]));
+        if (pre < 1.0f || !(wave_max(top) >= kLargest)) break;
+        pre = 0x1p-60f;
+    }
+    if (pre < 1.0f) {
+        // m + 60 is rounded; what that adds to 60 the weights leave off again.
+        const float raised = m + 60.0f;
+        const double off = static_cast<double>(m) - static_cast<double>(raised) + 60.0;
+        const float by = __builtin_amdgcn_exp2f(static_cast<float>(off));
+        m = raised;
+        l *= by * pre;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] *= by;
     }
 }
 
@@ -732,6 +754,7 @@ __device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& 
         }
     }
     l = sum32(sum16(l));
+    constexpr float kMost = NT == 3 ? kLargest : INFINITY;  // fp16's sums stay below 2^61
     float low = INFINITY;
 #pragma unroll
     for (int y = 0; y < VU; ++y)
@@ -739,7 +762,7 @@ __device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& 
         for (int r = 0; r < 4; ++r) {
             const int d = VU * (4 * g + r) + y;
             const float x = fabsf(o[y][r]);
-            bad |= d < D && !(x < INFINITY);
+            bad |= d < D && !(x < kMost);
             low = d < D ? fminf(low, x) : low;
         }
     // fp32 values that dropped bits, worth up to 2^-134 each, beside a sum so
@@ -1088,6 +1111,7 @@ __device__ __forceinline__ void wide_item(const PagedAttnArgs& a, const Item& it
     __syncthreads();
     if (idle) return;
     l = sum32(l);
+    constexpr float kMost = NT == 3 ? kLargest : INFINITY;
     float low = INFINITY;
 #pragma unroll
     for (int u = 0; u < DU; ++u)
@@ -1095,7 +1119,7 @@ __device__ __forceinline__ void wide_item(const PagedAttnArgs& a, const Item& it
         for (int r = 0; r < 16; ++r) {
             const int d = DU * (8 * (r / 4) + 4 * h + r % 4) + u;
             const float x = fabsf(o[u][r]);
-            bad |= d < D && !(x < INFINITY);
+            bad |= d < D && !(x < kMost);
             low = d < D ? fminf(low, x) : low;
         }
     if constexpr (KT == 3) bad |= v_lost && low < 0x1p-50f;

@@ -127,3 +127,21 @@ def test_many_small_weights(dtype, rows):
         want = s / (1 + s)
         tol = want * (n + r + 200) * 2.0 ** -24 + (n + r) * 2.0 ** -39 * (dtype == "f16")
         assert float((got[r] - want).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads, kv, D", [(4, 2, 64), (8, 1, 128), (2, 1, 256)])
+def test_values_near_the_types_largest(dtype, heads, kv, D):
+    """An output is a mean of values, so it is finite where they are, though a
+    sum of them is not; other heads' ordinary values stay as exact as ever."""
+    b = Batch(em, heads, kv, D, 16, [(100, 1), (20, 40), (3000, 1), (4000, 12), (0, 1), (64, 70)],
+              dtype, seed=93)
+    vv = b.view(b.vc)
+    big = (1.0 + torch.rand(vv.shape, generator=torch.Generator().manual_seed(94))) * 2.0 ** 126
+    vv[..., 0, :] = big[..., 0, :].to(vv.dtype)
+    check(b)
+    b.q()[:] *= 20.0  # a few positions take all the weight
+    b.qkv = b.qkv.cpu()
+    for name in ("table", "starts", "lengths", "kc", "vc"):
+        setattr(b, name, getattr(b, name).cpu())
+    check(b)
