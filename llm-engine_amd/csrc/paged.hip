@@ -62,7 +62,7 @@ struct AppendArgs {
 // Cosine and sine of an angle formed in 64 bits, rounded to fp32 once: the
 // angle less the nearest multiple of pi / 2 (held as a sum of two doubles, so
 // that 2^31 quarter turns leave the remainder good to 2^-75), then the Taylor
-// series of both, whose first terms left out are below 2^-37 of the sum's
+// series of both, whose first terms left out are below 2^-36 of the sum's
 // leading term at pi / 4, and the quarter's signs.
 __device__ __forceinline__ void cos_sin(double angle, float& c, float& s) {
     constexpr double kTwoOverPi = 0.63661977236758134308;
