@@ -151,3 +151,27 @@ def test_u_from_one_is_one_less_2_to_minus_53(R, V, kw, u):
     for r in range(R):
         want = int(behind[r] if far[r] == 30.0 else heavy[r])
         check(x, tok, lp, weights(x[r], 1.0), want, r)
+
+
+@pytest.mark.parametrize("p", [0.6, 0.9, 0.999])
+@pytest.mark.parametrize("R, V", SPREADS)
+def test_the_first_token_top_p_keeps(R, V, p):
+    """Rows of two or three tokens, and rows of many whose kept tokens are a
+    list or the row itself: the first of them at u = 0."""
+    rng = np.random.default_rng(R + 3 * V)
+    x = two_or_three(R, V, rng)
+    x[::2] = rng.normal(0, 1.0, (len(x[::2]), V)).astype(np.float32)
+    x[::4, rng.integers(0, V, 5)] += 12.0
+    tok, lp = draw(x, 0.0, top_p=p)
+    for r in range(R):
+        w = weights(x[r], 1.0)
+        order = np.lexsort((np.arange(V), -x[r]))
+        run = np.cumsum(w[order])
+        kept = order[:int((run < float(np.float32(p)) * run[-1]).sum()) + 1]
+        want = int(kept.min())
+        assert want != int(kept[-1]) or kept.size < 200  # not the border's own
+        only = np.zeros(V)
+        only[kept] = w[kept]
+        assert tok[r] == want, (r, tok[r], want)
+        l = math.log(only[want] / only.sum())
+        assert abs(lp[r] - l) <= 2.0 ** -24 * abs(l) + 2.0 ** -20, (r, lp[r], l)
