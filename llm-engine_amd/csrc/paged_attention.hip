@@ -462,7 +462,7 @@ __device__ __forceinline__ void plain_column(const PagedAttnArgs& a, int seq, in
 // Nothing is staged in LDS: 16 KB a wave are in flight (keys are loaded again
 // right after their product, values after theirs), which 8 waves a CU need to
 // keep HBM busy. Bound by the cache's bytes: 64 rows at 500 to 4000 positions (32
-// heads on 8 of 128, bf16) 135 us for 641 MB, 2 at 70001 to 131070 (fp16) 173 us
+// heads on 8 of 128, bf16) 136 us for 641 MB, 2 at 70001 to 131070 (fp16) 171 us
 // for 954 MB.
 template <class T, int DP>
 struct Few {
@@ -838,7 +838,7 @@ __device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& 
 // written to LDS after them (fp32: split into its three terms there). Bound by
 // the matrix cores, three products a multiply-add for bf16 and six for fp32,
 // beside the softmax of the other workgroup on the CU: 2048 rows of 32 heads on 8
-// of 128 behind 6100 positions (bf16) 663 us, 1076 TFLOP/s of products (16 columns
+// of 128 behind 6100 positions (bf16) 667 us, 1070 TFLOP/s of products (16 columns
 // an item: 1119 us).
 template <class T, int DP>
 struct Wide {
@@ -1384,7 +1384,8 @@ void run_paged_attention(PagedAttnArgs a, const em_paged_shape& s, float* scratc
     a.min_wide = s.type == EM_CACHE_F32 ? 192 : 512;
     // With two workgroups on a CU a wide item takes 175 ns a position of heads of
     // 128 (fp32; bf16 96, fp16 75), a narrow one that reads at HBM's rate 50 (fp32
-    // 100, of which the cache holds some).
+    // 100, of which the cache holds some). Measured at that head size alone; at
+    // others the ratio is assumed, both items' work being linear in it.
     a.wide_cost = s.type == EM_CACHE_F32 ? 3.0f : s.type == EM_CACHE_BF16 ? 2.0f : 1.5f;
     a.part_units = partial_units(s, rows);
     a.part_o = scratch;

@@ -20,9 +20,9 @@
 // rows of up to 32765 are read once, into LDS, longer ones once a pass (greedy and
 // unfiltered ones once in all). Not bound by the logits' bytes but by the passes
 // of a workgroup one behind the other: 1 x 32000 with top-k of 40 15 us, with
-// top-p of 0.9 34 (four passes over LDS, the 64-bit weights in two of them); 256 x
-// 131072 unfiltered 47 us (its weights 36), with min-p 60 to 70, greedy 27, where
-// a copy's rate would take 26.
+// top-p of 0.9 32 (four passes over LDS, the 64-bit weights in two of them); 256 x
+// 131072 unfiltered 43 us (weights, for the most part), with min-p 60, greedy 25,
+// where a copy's rate would take 26.
 #include <algorithm>
 #include <cmath>
 
@@ -90,7 +90,7 @@ __device__ constexpr double kRoot[2 * kRoots] = {
 // first term left out is below 2^-48). The whole part of z is read from the
 // low bits of z + 1.5 2^52 and added to the exponent's, so that of the
 // instructions only the conversion of x is not a 64-bit add or multiply-add
-// (9 ns per 1024 weights a CU with floor, ldexp and a 16-entry table: 14).
+// (floor, ldexp and a 16-entry table take half as long again).
 struct Weigh {
     float top;
     bool endless;  // top is +inf: its tokens share all the weight
@@ -956,7 +956,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs a
 // the caller's scratch by integer atomics, and a last launch of one workgroup a
 // row that draws. Rows that this does not fit (a logit of +inf, a border bin of
 // more than kList) are done by that workgroup alone, as above. Calls without
-// top-k only. 7 x 100003 with top-p: 3.3, 14, 8.6 and 19 us, waiting for the slices'
+// top-k only. 7 x 100003 with top-p: 3.8, 14, 8.9 and 17 us, waiting for the slices'
 // atomics and, a workgroup a row, for its own reads and sums.
 
 constexpr int kSliceThreads = 256;
