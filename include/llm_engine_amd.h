@@ -324,8 +324,9 @@ size_t em_paged_attention_scratch_floats(const em_paged_shape* s, size_t n_seqs,
  * output, whatever their slots hold. A row that sees nothing gets zeros. A row
  * past the table's last position sees the table's, by the query it is given
  * (append leaves that one alone): lengths[s] belongs within the table.
- * Sums are fp32; over an fp16 cache a weight below 2^-17 of the row's largest is
- * held to 2^-39 of that, others of every type to 2^-22 of themselves.
+ * Sums are fp32. Queries and weights enter the products to 2^-22 of themselves or
+ * better; over an fp16 cache small query dims may shift a score by 2^-20 in all (in
+ * log2 units) and a weight is held to 2^-39 of the row's largest where that is more.
  * Scratch is the caller's, used by this call alone until it has run; it needs
  * no zero fill. Results are bit-identical across calls of one shape, batch
  * and row count. Pointers 16-byte aligned, row strides multiples of 4. */
