@@ -357,7 +357,8 @@ size_t em_sample_scratch_bytes(size_t rows, size_t vocab);
  *   tokens[r]   the lowest i, in index order, with the kept weights up to and
  *               including i above u times their sum
  *   logprobs[r] ln(w_token / that sum); NULL: not wanted.
- * Weights are formed in 64 bits, those below e^-60 of the largest count as 0;
+ * Weights are formed in 64 bits, those below e^-60 of the largest count as 0 (the
+ * logit where that lies is rounded to fp32);
  * top-p's sums are integers of 2^-42 or finer (for a vocabulary of up to 2^20;
  * 2^-44 for 2^18), others are added in 64 bits in a fixed order, so timing
  * never changes a result. A NaN or -inf logit is never drawn; logits of +inf share
